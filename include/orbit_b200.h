@@ -352,6 +352,68 @@ int orbit_cp_state_pack(const float* dA, float* record, int B, int L, int HR, in
 int orbit_cp_state_combine(const float* records, int64_t stride, int world, int rank, int64_t n_state, int per_head, int BHR,
                            int backward, float* out, void* stream);
 
+/* ---- linear attention with a constant decay for each head -----------------------------------------------------------
+ *   S_t = a S_{t-1} + v_t k_t^T,   y_t = scale S_t q_t,   a = exp(log_decay[h]),   S [B, H, Dv, Dk] fp32 (NULL state0 = zeros)
+ * q, k [B, L, H, Dk], v, y [B, L, H, Dv] in the IO dtype with element strides (batch, token, head; the last axis is dense);
+ * log_decay [H] fp32, at most 0, a constant (no gradient).  Head widths 1..256; bfloat16 with widths that are multiples of 8 up
+ * to 128, 16-byte aligned pointers and strides that are multiples of 8 runs on tcgen05 tiles, everything else on fp32 kernels.
+ * Backward reads q, k, v, dy, state0 and dstate1 (gradient of the state after the sequence, NULL = zeros), writes dq, dk, dv
+ * and dstate0 (NULL = not wanted).  `status` (device int or NULL) is set if a bounded device wait gave up.  L = 0 passes the
+ * state through.  Outputs must not overlap inputs.  No counterpart in the reference, whose scans share their maps over heads
+ * and take a decay for each token. */
+typedef struct orbit_la_args {
+  int B, L, H, Dk, Dv;
+  float scale;
+  const void* q;  int64_t q_bs, q_ls, q_hs;
+  const void* k;  int64_t k_bs, k_ls, k_hs;
+  const void* v;  int64_t v_bs, v_ls, v_hs;
+  const float* log_decay;
+  const float* state0;        /* [B, H, Dv, Dk] or NULL                                                             */
+  void* y;        int64_t y_bs, y_ls, y_hs;
+  float* state1;              /* out [B, H, Dv, Dk] or NULL                                                         */
+  /* backward */
+  const void* dy; int64_t dy_bs, dy_ls, dy_hs;
+  const float* dstate1;       /* [B, H, Dv, Dk] or NULL                                                             */
+  void* dq;       int64_t dq_bs, dq_ls, dq_hs;
+  void* dk;       int64_t dk_bs, dk_ls, dk_hs;
+  void* dv;       int64_t dv_bs, dv_ls, dv_hs;
+  float* dstate0;             /* out [B, H, Dv, Dk] or NULL                                                         */
+  void* workspace; int64_t workspace_bytes;
+  int* status;
+} orbit_la_args;
+int64_t orbit_la_workspace_bytes(const orbit_la_args* a, int backward, int dtype);
+int orbit_la_fwd(const orbit_la_args* a, int dtype, void* stream);
+int orbit_la_bwd(const orbit_la_args* a, int dtype, void* stream);
+/* One token (decode): q, k [B, H, Dk], v [B, H, Dv] with (batch, head) strides, y [B, H, Dv] contiguous; state1 may be state0. */
+int orbit_la_step(const void* q, int64_t q_bs, int64_t q_hs, const void* k, int64_t k_bs, int64_t k_hs, const void* v,
+                  int64_t v_bs, int64_t v_hs, const float* log_decay, const float* state0, float* state1, void* y, int B,
+                  int H, int Dk, int Dv, float scale, int dtype, void* stream);
+
+/* ---- the norms around a block: post-norm, gate, residual scale and add, pre-norm of what follows -----------------------
+ *   u = h * rsqrt(mean(h^2) + eps) * w_post (w_post NULL: u = h);   m = u * sigmoid(gate) (gate NULL: m = u)
+ *   r = x + scale * m (scale NULL: 1);   n = r * rsqrt(mean(r^2) + eps) * w_pre (w_pre NULL: n is not formed)
+ * x, h, gate [M, D] with row strides, r, n and every gradient [M, D] contiguous, IO dtype; scale, w_post, w_pre [D] fp32.
+ * rstd_h / rstd_r [M] fp32: out of the forward (NULL: not kept), in to the backward.  Backward: dr or dn may be NULL (zeros);
+ * dscale, dw_post, dw_pre [D] fp32 or NULL are reduced in a fixed order through `workspace`.  Beside orbit_gate_norm_*, whose
+ * norm and gate it joins with the residual of src/orbit_ssm/model.py:51-118. */
+int orbit_block_norm_fwd(const void* x, int64_t x_row_stride, const void* h, int64_t h_row_stride, const void* gate,
+                         int64_t gate_row_stride, const float* scale, const float* w_post, const float* w_pre, void* r,
+                         void* n, float* rstd_h, float* rstd_r, int64_t M, int D, float eps, int dtype, void* stream);
+int64_t orbit_block_norm_bwd_workspace_bytes(int64_t M, int D);
+int orbit_block_norm_bwd(const void* x, int64_t x_row_stride, const void* h, int64_t h_row_stride, const void* gate,
+                         int64_t gate_row_stride, const float* scale, const float* w_post, const float* w_pre,
+                         const float* rstd_h, const float* rstd_r, const void* dr, const void* dn, void* dx, void* dh,
+                         void* dgate, float* dscale, float* dw_post, float* dw_pre, void* workspace, int64_t workspace_bytes,
+                         int64_t M, int D, int dtype, void* stream);
+
+/* ---- activations in eight bits ------------------------------------------------------------------------------------------
+ * x [M, D] (row stride in elements) -> q [M, D] signed bytes, exponent [M, ceil(D / 32)] bytes (e + 127 for each 32
+ * consecutive elements of a row): x ~ q 2^e with the least e >= -126 for which the group's largest |x| rounds to at most 127.
+ * Codes of the largest step 2^122 end at +-63 (the restored value stays finite).  The code -128 marks a non-finite element and is restored as NaN.  Restoring is exact in either dtype.  No counterpart in the
+ * reference. */
+int orbit_act_pack(const void* x, int64_t x_row_stride, void* q, void* exponent, int64_t M, int D, int dtype, void* stream);
+int orbit_act_unpack(const void* q, const void* exponent, void* x, int64_t M, int D, int dtype, void* stream);
+
 /* ---- diagnostics ---------------------------------------------------------------------------------------------
  * One 128 x N x K tcgen05 tile through the same TMA boxes, shared-memory descriptors and TMEM read-out as the scan
  * kernels: D[128, N] fp32 = op(A) * op(B), A and B bfloat16.  mode bit 0: A given as [K, 128] (M contiguous) instead

@@ -82,6 +82,25 @@ class HmTailArgs(C.Structure):
     ]
 
 
+class LaArgs(C.Structure):
+    """Mirror of ``orbit_la_args`` (include/orbit_b200.h); field order and types must match the header."""
+    _fields_ = (
+        [(n, C.c_int) for n in ("B", "L", "H", "Dk", "Dv")] + [("scale", C.c_float)]
+        + [("q", C.c_void_p), ("q_bs", C.c_int64), ("q_ls", C.c_int64), ("q_hs", C.c_int64)]
+        + [("k", C.c_void_p), ("k_bs", C.c_int64), ("k_ls", C.c_int64), ("k_hs", C.c_int64)]
+        + [("v", C.c_void_p), ("v_bs", C.c_int64), ("v_ls", C.c_int64), ("v_hs", C.c_int64)]
+        + [("log_decay", C.c_void_p), ("state0", C.c_void_p)]
+        + [("y", C.c_void_p), ("y_bs", C.c_int64), ("y_ls", C.c_int64), ("y_hs", C.c_int64)]
+        + [("state1", C.c_void_p)]
+        + [("dy", C.c_void_p), ("dy_bs", C.c_int64), ("dy_ls", C.c_int64), ("dy_hs", C.c_int64)]
+        + [("dstate1", C.c_void_p)]
+        + [("dq", C.c_void_p), ("dq_bs", C.c_int64), ("dq_ls", C.c_int64), ("dq_hs", C.c_int64)]
+        + [("dk", C.c_void_p), ("dk_bs", C.c_int64), ("dk_ls", C.c_int64), ("dk_hs", C.c_int64)]
+        + [("dv", C.c_void_p), ("dv_bs", C.c_int64), ("dv_ls", C.c_int64), ("dv_hs", C.c_int64)]
+        + [("dstate0", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("status", C.c_void_p)]
+    )
+
+
 HM_CHUNK = 32     # checkpoint interval (tokens) the HybridMamba backward kernel is written for
 
 _P, _I, _L, _F = C.c_void_p, C.c_int, C.c_int64, C.c_float
@@ -118,6 +137,15 @@ SIGNATURES = {
     "orbit_cp_state_pack_workspace_bytes": (_L, [_I, _I, _I]),
     "orbit_cp_state_pack": (_I, [_P, _P, _I, _I, _I, _L, _P, _L, _P]),
     "orbit_cp_state_combine": (_I, [_P, _L, _I, _I, _L, _I, _I, _I, _P, _P]),
+    "orbit_la_workspace_bytes": (_L, [_P, _I, _I]),
+    "orbit_la_fwd": (_I, [_P, _I, _P]),
+    "orbit_la_bwd": (_I, [_P, _I, _P]),
+    "orbit_la_step": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P]),
+    "orbit_block_norm_fwd": (_I, [_P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _L, _I, _F, _I, _P]),
+    "orbit_block_norm_bwd_workspace_bytes": (_L, [_L, _I]),
+    "orbit_block_norm_bwd": (_I, [_P, _L, _P, _L, _P, _L] + [_P] * 14 + [_L, _L, _I, _I, _P]),
+    "orbit_act_pack": (_I, [_P, _L, _P, _P, _L, _I, _I, _P]),
+    "orbit_act_unpack": (_I, [_P, _P, _P, _L, _I, _I, _P]),
     "orbit_selftest_umma": (_I, [_P, _P, _P, _I, _I, _I, _P, _P]),
     "orbit_selftest_wait_timeout": (_I, [_P, _I, _P]),
 }

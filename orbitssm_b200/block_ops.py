@@ -1,0 +1,281 @@
+"""Operators around a block: the norms before and after it fused with gate, residual scale and residual add
+(`block_norm`), and the 8-bit form in which a block's input waits for the backward pass (`pack_activation`,
+`unpack_activation`).  `ResidualBlock` and `BlockStack` call them; they run `orbit_block_norm_*` and `orbit_act_*` of the
+C-ABI library on the current stream of the tensors' device.
+"""
+from __future__ import annotations
+
+import contextlib
+from typing import NamedTuple
+
+import torch
+
+from . import _lib, ops
+
+PACK_GROUP = 32      # elements of a row that share one exponent
+
+_DT = ops._DT
+_NULL = contextlib.nullcontext()
+
+
+def device_of(who, *tensors):
+    """The one CUDA device the tensors live on; a CPU tensor or a second device is refused by name."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            ops._require_cuda(who, t)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{who}: tensors on {dev} and {t.device}; all of them have to be on one device")
+    return dev
+
+
+def on(device):
+    """Context in which `device` is the current one (kernels launch there, whatever device the caller had current)."""
+    return _NULL if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _count(launches):
+    ops.LAUNCHES += launches
+
+
+def io_code(who, t):
+    code = _DT.get(t.dtype)
+    if code is None:
+        raise NotImplementedError(f"{who}: activations must be float32 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+# ----------------------------------------------------------------------------------------------------
+#  norms around a block
+# ----------------------------------------------------------------------------------------------------
+def _rows_of(t, D):
+    """[..., D] as [M, D] rows of one stride with a dense last axis; copied only where no view is one."""
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t
+    if t.is_contiguous():
+        return t.view(-1, D)
+    if t.stride(-1) != 1:
+        return t.contiguous().view(-1, D)
+    t = ops._as_rows(t, D)
+    return t if t.stride(1) == 1 else t.contiguous()
+
+
+def _stride(t):
+    return t.shape[1] if t.shape[0] <= 1 else t.stride(0)      # the stride of a single row is never used
+
+
+def block_norm_fwd(x, h, gate, scale, w_post, w_pre, eps, keep):
+    """x, h, gate [M, D] (gate may be None), weights fp32 [D] or None -> (r, n | None, rstd_h | None, rstd_r | None);
+    the rstd are kept where `keep`."""
+    dev = device_of("block_norm", x, h, gate, scale, w_post, w_pre)
+    M, D = x.shape
+    r = torch.empty((M, D), device=dev, dtype=x.dtype)
+    n = torch.empty((M, D), device=dev, dtype=x.dtype) if w_pre is not None else None
+    rh = torch.empty((M,), device=dev, dtype=torch.float32) if keep and w_post is not None else None
+    rr = torch.empty((M,), device=dev, dtype=torch.float32) if keep and w_pre is not None else None
+    if M:
+        with on(dev), ops._timed("block_norm_fwd", 1):
+            _lib.check(_lib.load().orbit_block_norm_fwd(
+                x.data_ptr(), _stride(x), h.data_ptr(), _stride(h), _ptr(gate), 0 if gate is None else _stride(gate),
+                _ptr(scale), _ptr(w_post), _ptr(w_pre), r.data_ptr(), _ptr(n), _ptr(rh), _ptr(rr), M, D, eps,
+                _DT[x.dtype], raw_stream(dev)), "orbit_block_norm_fwd")
+    return r, n, rh, rr
+
+
+def block_norm_bwd(x, h, gate, scale, w_post, w_pre, rstd_h, rstd_r, dr, dn, want_sums=True):
+    """Gradients of `block_norm_fwd`: (dx, dh, dgate | None, dscale | None, dw_post | None, dw_pre | None); dr or dn may
+    be None (zeros).  Without `want_sums` the three column sums are left out."""
+    dev = device_of("block_norm", x, h, gate, scale, w_post, w_pre, dr, dn)
+    M, D = x.shape
+    f32 = torch.float32
+    dx = torch.empty((M, D), device=dev, dtype=x.dtype)
+    dh = torch.empty_like(dx)
+    dg = torch.empty_like(dx) if gate is not None else None
+    sums = [torch.empty((D,), device=dev, dtype=f32) if (want_sums and w is not None) else None for w in (scale, w_post, w_pre)]
+    lib = _lib.load()
+    nbytes, ws = 0, None
+    if any(s is not None for s in sums):
+        nbytes = lib.orbit_block_norm_bwd_workspace_bytes(M, D)
+        ws = torch.empty((nbytes,), device=dev, dtype=torch.uint8)
+    with on(dev), ops._timed("block_norm_bwd", (2 if ws is not None else 1) if M else 0):
+        _lib.check(lib.orbit_block_norm_bwd(
+            x.data_ptr(), _stride(x), h.data_ptr(), _stride(h), _ptr(gate), 0 if gate is None else _stride(gate), _ptr(scale),
+            _ptr(w_post), _ptr(w_pre), _ptr(rstd_h), _ptr(rstd_r), _ptr(dr), _ptr(dn), dx.data_ptr(), dh.data_ptr(), _ptr(dg),
+            _ptr(sums[0]), _ptr(sums[1]), _ptr(sums[2]), _ptr(ws), nbytes, M, D, _DT[x.dtype], raw_stream(dev)),
+            "orbit_block_norm_bwd")
+    return (dx, dh, dg, *sums)
+
+
+class BlockNormFn(torch.autograd.Function):
+    """(r, n) of `block_norm`; n is None without a pre-norm weight."""
+
+    @staticmethod
+    def forward(ctx, x, h, gate, scale, w_post, w_pre, eps):
+        D = x.shape[-1]
+        x2, h2 = _rows_of(x, D), _rows_of(h, D)
+        g2 = None if gate is None else _rows_of(gate, D)
+        s32, wo, wi = ops._f32(scale), ops._f32(w_post), ops._f32(w_pre)
+        keep = any(ctx.needs_input_grad)
+        r, n, rh, rr = block_norm_fwd(x2, h2, g2, s32, wo, wi, eps, keep)
+        if keep:
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(x2, h2, g2, s32, wo, wi, rh, rr)
+            ctx.meta = (x.shape, [None if t is None else t.dtype for t in (scale, w_post, w_pre)])
+        return r.view(x.shape), None if n is None else n.view(x.shape)
+
+    @staticmethod
+    @ops.first_order_only("block norm")
+    def backward(ctx, dr, dn):
+        if dr is None and dn is None:
+            return (None,) * 7
+        x2, h2, g2, s32, wo, wi, rh, rr = ctx.saved_tensors
+        shape, dts = ctx.meta
+        D = shape[-1]
+        dr2 = None if dr is None else dr.contiguous().view(-1, D)
+        dn2 = None if dn is None else dn.contiguous().view(-1, D)
+        need = ctx.needs_input_grad
+        dx, dh, dg, *sums = block_norm_bwd(x2, h2, g2, s32, wo, wi, rh, rr, dr2, dn2, want_sums=any(need[3:6]))
+        out = [dx.view(shape) if need[0] else None, dh.view(shape) if need[1] else None,
+               dg.view(shape) if need[2] else None]
+        out += [s.to(dt) if (need[3 + i] and s is not None) else None for i, (s, dt) in enumerate(zip(sums, dts))]
+        return (*out, None)
+
+
+def block_norm(x, h, *, gate=None, scale=None, post_weight=None, pre_weight=None, eps=1e-5):
+    """Joins a block's output `h` to the residual stream `x` and normalises the sum for what follows, in one kernel:
+
+        u = rms_norm(h) * post_weight        (u = h without `post_weight`)
+        r = x + scale * u * sigmoid(gate)    (no gate factor without `gate`, scale 1 without `scale`)
+        n = rms_norm(r) * pre_weight         (None without `pre_weight`)
+
+    x, h, gate: [..., D] of one shape and dtype (float32 or bfloat16; a column slice of a wider buffer is read in place);
+    scale, post_weight, pre_weight: [D].  Returns (r, n) in the dtype of x; arithmetic, norms and the weights' gradients are
+    float32, and n is formed from the unrounded r.  First-order differentiable in every tensor argument."""
+    who = "block_norm"
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{who}: expected x [..., D] with D > 0, got {tuple(x.shape)}")
+    io_code(who, x)
+    for name, t in (("h", h), ("gate", gate)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"{who}: {name} must have the shape and dtype of x ({tuple(x.shape)}, {x.dtype}), got "
+                             f"{tuple(t.shape)}, {t.dtype}")
+    for name, t in (("scale", scale), ("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if t is not None and (t.dim() != 1 or t.shape[0] != x.shape[-1] or not t.is_floating_point()):
+            raise ValueError(f"{who}: {name} must be a floating [{x.shape[-1]}] vector, got {tuple(t.shape)}, {t.dtype}")
+    if not eps >= 0:
+        raise ValueError(f"{who}: eps must be at least 0, got {eps!r}")
+    device_of(who, x, h, gate, scale, post_weight, pre_weight)
+    return BlockNormFn.apply(x, h, gate, scale, post_weight, pre_weight, float(eps))
+
+
+# ----------------------------------------------------------------------------------------------------
+#  activations in eight bits
+# ----------------------------------------------------------------------------------------------------
+class PackedActivation(NamedTuple):
+    """An activation in eight bits: x ~ q * 2^(exponent - 127), one exponent for each 32 consecutive elements of a row."""
+    q: torch.Tensor           # int8, the activation's shape
+    exponent: torch.Tensor    # uint8 [..., ceil(D / 32)]
+    dtype: torch.dtype        # what the activation was
+
+    @property
+    def nbytes(self):
+        return self.q.numel() + self.exponent.numel()
+
+
+def pack_activation(x):
+    """x [..., D] (float32 or bfloat16, a dense last axis) -> `PackedActivation`: a signed byte an element and one power of
+    two for each 32 elements of a row, the least under which the group's largest element rounds to at most 127 (never below
+    2^-126).  Rounding is to nearest, ties to even: off by at most half a step, and a step is at most 1/64 of the group's
+    largest element (values within 2^122 of the type's largest are off by up to a step, so as to stay finite).  A non-finite element is restored as NaN and leaves its group's scale alone.  Not differentiable."""
+    who = "pack_activation"
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{who}: expected x [..., D] with D > 0, got {tuple(x.shape)}")
+    code = io_code(who, x)
+    x = x.detach()
+    dev = device_of(who, x)
+    D = x.shape[-1]
+    x2 = _rows_of(x, D)
+    M = x2.shape[0]
+    q = torch.empty(x.shape, device=dev, dtype=torch.int8)
+    e = torch.empty((*x.shape[:-1], -(-D // PACK_GROUP)), device=dev, dtype=torch.uint8)
+    if M:
+        with on(dev), ops._timed("act_pack", 1):
+            _lib.check(_lib.load().orbit_act_pack(x2.data_ptr(), _stride(x2), q.data_ptr(), e.data_ptr(), M, D, code, raw_stream(dev)),
+                       "orbit_act_pack")
+    return PackedActivation(q, e, x.dtype)
+
+
+def unpack_activation(packed, dtype=None):
+    """The activation a `PackedActivation` stands for, in `dtype` (default: its own; exact in float32 and in bfloat16)."""
+    who = "unpack_activation"
+    q, e, own_dtype = packed
+    dtype = own_dtype if dtype is None else dtype
+    if dtype not in _DT:
+        raise NotImplementedError(f"{who}: activations must be float32 or bfloat16, got {dtype}")
+    if q.dtype != torch.int8 or e.dtype != torch.uint8 or q.dim() < 1 or q.shape[-1] == 0 \
+            or tuple(e.shape) != (*q.shape[:-1], -(-q.shape[-1] // PACK_GROUP)):
+        raise ValueError(f"{who}: expected int8 q [..., D] with uint8 exponents [..., ceil(D / {PACK_GROUP})], got {q.dtype} "
+                         f"{tuple(q.shape)} with {e.dtype} {tuple(e.shape)}")
+    dev = device_of(who, q, e)
+    q, e = q.contiguous(), e.contiguous()
+    x = torch.empty(q.shape, device=dev, dtype=dtype)
+    D = q.shape[-1]
+    if q.numel():
+        with on(dev), ops._timed("act_unpack", 1):
+            _lib.check(_lib.load().orbit_act_unpack(q.data_ptr(), e.data_ptr(), x.data_ptr(), q.numel() // D, D, _DT[dtype],
+                                                    raw_stream(dev)), "orbit_act_unpack")
+    return x
+
+
+class CheckpointFn(torch.autograd.Function):
+    """``block(x)`` without keeping what the block's backward needs: its input waits in eight bits, and the backward pass
+    restores it, runs the block again and differentiates that run."""
+
+    @staticmethod
+    def forward(ctx, block, x, *params):
+        ctx.block = block
+        ctx.amp = (torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda"))
+        ctx.versions = [p._version for p in params]
+        packed = pack_activation(x)
+        ctx.dtype = x.dtype
+        with torch.no_grad():
+            y = block(x)
+        ctx.save_for_backward(packed.q, packed.exponent, *params)
+        return y
+
+    @staticmethod
+    @ops.first_order_only("8-bit activation checkpoint")
+    def backward(ctx, dy):
+        q, e, *params = ctx.saved_tensors
+        if [p._version for p in params] != ctx.versions:
+            raise RuntimeError("8-bit activation checkpoint: a parameter of the block was changed in place between the forward "
+                               "and the backward pass; the block cannot be run again as it was")
+        x = unpack_activation(PackedActivation(q, e, ctx.dtype)).requires_grad_(ctx.needs_input_grad[1])
+        wanted = [p for p, need in zip(params, ctx.needs_input_grad[2:]) if need]
+        ins = ([x] if ctx.needs_input_grad[1] else []) + wanted
+        enabled, dtype = ctx.amp
+        with torch.enable_grad(), torch.autocast("cuda", dtype=dtype, enabled=enabled, cache_enabled=False):
+            y = ctx.block(x)
+        grads = list(torch.autograd.grad(y, ins, dy, allow_unused=True))
+        dx = grads.pop(0) if ctx.needs_input_grad[1] else None
+        return (None, dx, *[grads.pop(0) if need else None for need in ctx.needs_input_grad[2:]])
+
+
+def checkpoint_block(block, x):
+    """``block(x)`` under an 8-bit activation checkpoint (see `CheckpointFn`); an ordinary call where no gradient is wanted."""
+    params = [p for p in block.parameters() if p.requires_grad]
+    if not torch.is_grad_enabled() or not (x.requires_grad or params):
+        return block(x)
+    return CheckpointFn.apply(block, x, *params)

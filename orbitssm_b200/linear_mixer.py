@@ -1,0 +1,415 @@
+"""Linear attention with a constant decay for each head: the operators `linear_attention` (a sequence, differentiable,
+with the state carried in and out) and `linear_attention_step` (one token), and the mixer layer `LinearAttention` on them.
+
+    S_t = a S_{t-1} + v_t k_t^T,    y_t = scale S_t q_t,    a = exp(log_decay[head])
+
+Where the SSD scan shares its maps over the heads and takes a decay for each token, here every head has keys and queries of
+its own and one decay.  The state [B, H, Dv, Dk] is float32; its layout is that of the other layers' ``hidden_state``
+[B, H, P, N] (channel, state row).
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from dataclasses import asdict, dataclass
+
+import torch
+import torch.nn as nn
+
+from . import _lib, ops
+from .block_ops import device_of, io_code, on, raw_stream
+from .config import BACKENDS, PRECISIONS, _positive_int, _strict_from_dict, as_execution
+from .state import State, StateLifecycle
+
+
+# ----------------------------------------------------------------------------------------------------
+#  the operators
+# ----------------------------------------------------------------------------------------------------
+def _operand(t):
+    """`t` [B, L, H, D] as the kernels read it: a dense last axis; for bfloat16 heads of a multiple of 8 also 16-byte rows and no
+    overlapping (expanded) axes, so that the tensor-core tiles can load it.  Copied only where it is not so already."""
+    sb, sl, sh, sd = t.stride()
+    if sd != 1 and t.shape[3] > 1:
+        return t.contiguous()
+    if t.dtype == torch.bfloat16 and t.shape[3] % 8 == 0:
+        if t.data_ptr() % 16:
+            return t.clone(memory_format=torch.contiguous_format)
+        for n, s in ((t.shape[0], sb), (t.shape[1], sl), (t.shape[2], sh)):
+            if n > 1 and (s % 8 or s <= 0):
+                return t.contiguous()
+    return t
+
+
+def _strides(t):
+    """(batch, token, head) strides; an axis of one element, whose stride is never used, gets an aligned one."""
+    return tuple(s if n > 1 else 8 for n, s in zip(t.shape[:3], t.stride()[:3]))
+
+
+def _status(device):
+    if ("cuda", device.index) not in ops._STATUS and torch.cuda.is_current_stream_capturing():
+        return None                # the word must not be born in a graph's memory pool
+    return ops._status_word(device).data_ptr()
+
+
+def _args(q, k, v, log_decay, state, scale):
+    a = _lib.LaArgs()
+    a.B, a.L, a.H, a.Dk, a.Dv, a.scale = q.shape[0], q.shape[1], q.shape[2], q.shape[3], v.shape[3], scale
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_bs, a.q_ls, a.q_hs = _strides(q)
+    a.k_bs, a.k_ls, a.k_hs = _strides(k)
+    a.v_bs, a.v_ls, a.v_hs = _strides(v)
+    a.log_decay = log_decay.data_ptr()
+    if state is not None:
+        a.state0 = state.data_ptr()
+    a.status = _status(q.device)
+    return a
+
+
+def _workspace(a, bwd, code, device):
+    nbytes = _lib.load().orbit_la_workspace_bytes(C.byref(a), bwd, code)
+    if not nbytes:
+        return None
+    ws = torch.empty((nbytes,), device=device, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    return ws
+
+
+def la_fwd(q, k, v, log_decay, state, scale, want_state):
+    """Operands as `_operand` leaves them -> (y [B, L, H, Dv], state [B, H, Dv, Dk] | None)."""
+    dev = q.device
+    B, L, H, Dk = q.shape
+    Dv = v.shape[3]
+    y = torch.empty((B, L, H, Dv), device=dev, dtype=q.dtype)
+    new = torch.empty((B, H, Dv, Dk), device=dev, dtype=torch.float32) if want_state else None
+    if B == 0 or (L == 0 and not want_state):
+        return y, new
+    code = ops._DT[q.dtype]
+    with on(dev):
+        a = _args(q, k, v, log_decay, state, scale)
+        a.y = y.data_ptr()
+        a.y_bs, a.y_ls, a.y_hs = _strides(y)
+        if new is not None:
+            a.state1 = new.data_ptr()
+        ws = _workspace(a, 0, code, dev)  # noqa: F841 - alive until the launch is queued on this stream
+        with ops._timed("linear_attention_fwd", 1 if ws is None else 2):
+            _lib.check(_lib.load().orbit_la_fwd(C.byref(a), code, raw_stream(dev)), "orbit_la_fwd")
+    return y, new
+
+
+def la_bwd(q, k, v, log_decay, state, scale, dy, dstate, want_dstate0, outs=(None, None, None)):
+    """Gradients (dq, dk, dv, dstate0 | None); `outs` may name tensors (any strides, dense last axis) that receive dq, dk, dv."""
+    dev = q.device
+    dq, dk, dv = (o if o is not None else torch.empty(t.shape, device=dev, dtype=t.dtype) for o, t in zip(outs, (q, k, v)))
+    B, L, H, Dk = q.shape
+    ds0 = torch.empty((B, H, v.shape[3], Dk), device=dev, dtype=torch.float32) if want_dstate0 else None
+    if B == 0 or (L == 0 and not want_dstate0):
+        return dq, dk, dv, ds0
+    code = ops._DT[q.dtype]
+    with on(dev):
+        a = _args(q, k, v, log_decay, state, scale)
+        a.dy = dy.data_ptr()
+        a.dy_bs, a.dy_ls, a.dy_hs = _strides(dy)
+        if dstate is not None:
+            a.dstate1 = dstate.data_ptr()
+        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        a.dq_bs, a.dq_ls, a.dq_hs = _strides(dq)
+        a.dk_bs, a.dk_ls, a.dk_hs = _strides(dk)
+        a.dv_bs, a.dv_ls, a.dv_hs = _strides(dv)
+        if ds0 is not None:
+            a.dstate0 = ds0.data_ptr()
+        ws = _workspace(a, 1, code, dev)  # noqa: F841
+        with ops._timed("linear_attention_bwd", 1 if ws is None else 2):
+            _lib.check(_lib.load().orbit_la_bwd(C.byref(a), code, raw_stream(dev)), "orbit_la_bwd")
+    return dq, dk, dv, ds0
+
+
+class LinearAttentionFn(torch.autograd.Function):
+    """(y, state after the sequence | None).  `slots`: (GradArena, column-range index) of q, k and v, or None each."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, scale, want_state, slots):
+        q, k, v = _operand(q), _operand(k), _operand(v)
+        s0 = None if state is None else state.detach().contiguous()
+        y, new = la_fwd(q, k, v, log_decay, s0, scale, want_state)
+        if any(ctx.needs_input_grad):
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(q, k, v, log_decay, s0)
+            ctx.scale, ctx.slots = scale, slots
+        return y, new
+
+    @staticmethod
+    @ops.first_order_only("linear attention")
+    def backward(ctx, dy, dstate):
+        if dy is None and dstate is None:
+            return (None,) * 8
+        q, k, v, log_decay, s0 = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dy = torch.zeros(v.shape, device=v.device, dtype=v.dtype) if dy is None else _operand(dy)
+        dstate = None if dstate is None else dstate.contiguous()
+        outs = [None] * 3
+        if ctx.slots is not None:
+            for i, (t, slot) in enumerate(zip((q, k, v), ctx.slots)):
+                if slot is not None and need[i]:
+                    B, L, H, D = t.shape
+                    view = slot[0].view(slot[1], dy.new_empty((1,)).expand(B, L, H * D))     # a tensor of the range's shape
+                    if view is not None and _operand(view.unflatten(2, (H, D))).data_ptr() == view.data_ptr():
+                        outs[i] = view.unflatten(2, (H, D))
+        dq, dk, dv, ds0 = la_bwd(q, k, v, log_decay, s0, ctx.scale, dy, dstate, need[4] and s0 is not None, outs)
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, ds0 if need[4] else None,
+                None, None, None)
+
+
+def _check_operands(who, q, k, v, log_decay, state, lead):
+    """Shapes, dtypes and device of a call; `lead` names the axes before the heads."""
+    n = len(lead)
+    if q.dim() != n + 2 or k.shape != q.shape or v.dim() != n + 2 or v.shape[:-1] != q.shape[:-1]:
+        axes = ", ".join(lead)
+        raise ValueError(f"{who}: expected q, k [{axes}, H, Dk] and v [{axes}, H, Dv] (as many key heads as query heads: expand shared "
+                         f"heads), got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    code = io_code(who, q)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{who}: q, k and v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    H, Dk, Dv = q.shape[-2], q.shape[-1], v.shape[-1]
+    if H < 1 or not 1 <= Dk <= 256 or not 1 <= Dv <= 256:
+        raise NotImplementedError(f"{who}: at least one head, of widths 1..256, got H={H} Dk={Dk} Dv={Dv}")
+    if log_decay.dim() != 1 or log_decay.shape[0] != H or log_decay.dtype != torch.float32:
+        raise ValueError(f"{who}: log_decay must be float32 [{H}], got {log_decay.dtype} {tuple(log_decay.shape)}")
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{who}: log_decay is a constant of the layer; its gradient is not served (detach it)")
+    if state is not None and (tuple(state.shape) != (q.shape[0], H, Dv, Dk) or state.dtype != torch.float32):
+        raise ValueError(f"{who}: state must be float32 {(q.shape[0], H, Dv, Dk)}, got {state.dtype} {tuple(state.shape)}")
+    device_of(who, q, k, v, log_decay, state)
+    return code
+
+
+def _scale_of(who, scale, Dk):
+    if scale is None:
+        return Dk ** -0.5
+    scale = float(scale)
+    if not math.isfinite(scale) or scale == 0.0:
+        raise ValueError(f"{who}: scale must be finite and not zero, got {scale!r}")
+    return scale
+
+
+def linear_attention(q, k, v, log_decay, state=None, *, scale=None, return_state=False, _slots=None):
+    """y_t = scale S_t q_t over a sequence, with S_t = exp(log_decay) S_{t-1} + v_t k_t^T for each head.
+
+    q, k [B, L, H, Dk], v [B, L, H, Dv]: float32 or bfloat16, any strides (strided views with a dense last axis are read in
+    place); log_decay [H] float32, at most 0, a constant; state [B, H, Dv, Dk] float32 before the sequence (None: zeros);
+    scale: default Dk^-0.5.  Returns y [B, L, H, Dv] in the dtype of q, or (y, state after the sequence) with
+    `return_state`.  L may be 0.  First-order differentiable in q, k, v and state, through y and the returned state.
+
+    bfloat16 heads whose widths are multiples of 8 up to 128 run on tensor-core tiles: products of the unrounded inputs with the
+    scores or the state rounded once to bfloat16, float32 sums; the state itself is float32 throughout.  Other calls run on
+    float32 kernels.  Values are expected to be finite: a NaN or infinity may reach every output of its head and sequence."""
+    who = "linear_attention"
+    _check_operands(who, q, k, v, log_decay, state, ("B", "L"))
+    y, new = LinearAttentionFn.apply(q, k, v, log_decay.detach().contiguous(), state, _scale_of(who, scale, q.shape[-1]),
+                                     bool(return_state), _slots)
+    return (y, new) if return_state else y
+
+
+def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out_state=None):
+    """One token: q, k [B, H, Dk], v [B, H, Dv], state [B, H, Dv, Dk] float32 -> (y [B, H, Dv], state after the token).
+
+    `out_state` (contiguous float32 of the state's shape) receives the new state; it may be `state` itself.  For inference: not
+    differentiable (run `linear_attention` on a sequence of one token for gradients).  Everything else as there."""
+    who = "linear_attention_step"
+    if state is None:
+        raise ValueError(f"{who}: a state is required (zeros before the first token)")
+    code = _check_operands(who, q, k, v, log_decay, state, ("B",))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        raise ValueError(f"{who}: gradients are not served; use linear_attention on a sequence of one token, or torch.no_grad()")
+    if out_state is not None and (out_state.shape != state.shape or out_state.dtype != torch.float32 or not out_state.is_contiguous()
+                                  or out_state.device != state.device):
+        raise ValueError(f"{who}: out_state must be contiguous float32 {tuple(state.shape)} on {state.device}")
+    scale = _scale_of(who, scale, q.shape[-1])
+    B, H, Dk = q.shape
+    Dv, dev = v.shape[2], q.device
+    q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
+    state = state.contiguous()
+    if out_state is not None and out_state.data_ptr() != state.data_ptr() and _overlap(out_state, state):
+        raise ValueError(f"{who}: out_state overlaps state without being it")
+    new = torch.empty_like(state) if out_state is None else out_state
+    y = torch.empty((B, H, Dv), device=dev, dtype=q.dtype)
+    if B:
+        with on(dev), ops._timed("linear_attention_step", 1):
+            _lib.check(_lib.load().orbit_la_step(
+                q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                v.stride(1), log_decay.contiguous().data_ptr(), state.data_ptr(), new.data_ptr(), y.data_ptr(), B, H, Dk, Dv, scale, code,
+                raw_stream(dev)), "orbit_la_step")
+    return y, new
+
+
+def _overlap(a, b):
+    n = a.numel() * 4
+    return a.data_ptr() < b.data_ptr() + n and b.data_ptr() < a.data_ptr() + n
+
+
+# ----------------------------------------------------------------------------------------------------
+#  the layer
+# ----------------------------------------------------------------------------------------------------
+@dataclass(frozen=True)
+class LinearAttentionConfig:
+    """`LinearAttention` layer.  Heads have keys of `d_key` and values of `d_value` channels (default d_model / n_heads
+    each); head h forgets over a span that runs geometrically from `span_min` to `span_max` tokens: decay 1 - 1 / span."""
+    d_model: int
+    n_heads: int
+    d_key: int | None = None
+    d_value: int | None = None
+    span_min: float = 32.0
+    span_max: float = 4096.0
+    out_norm: bool = True
+    norm_eps: float = 1e-5
+
+    def __post_init__(self):
+        _positive_int(self.d_model, "d_model")
+        _positive_int(self.n_heads, "n_heads")
+        for name in ("d_key", "d_value"):
+            v = getattr(self, name)
+            if v is None:
+                if self.d_model % self.n_heads:
+                    raise ValueError(f"{name}: n_heads={self.n_heads} does not divide d_model={self.d_model}; give the head width")
+                object.__setattr__(self, name, self.d_model // self.n_heads)
+            elif _positive_int(v, name) > 256:
+                raise ValueError(f"{name} must be at most 256, got {v}")
+            if getattr(self, name) > 256:
+                raise ValueError(f"{name}={getattr(self, name)}: head widths go up to 256")
+        if not 1.0 < self.span_min <= self.span_max:
+            raise ValueError(f"spans must satisfy 1 < span_min <= span_max, got {self.span_min}, {self.span_max}")
+        if not isinstance(self.out_norm, bool):
+            raise TypeError("out_norm must be a bool")
+
+    def to_dict(self):
+        return asdict(self)
+
+    @classmethod
+    def from_dict(cls, d):
+        return _strict_from_dict(cls, d)
+
+
+class _OutNorm(nn.Module):
+    """Parameter holder of the output RMSNorm; the arithmetic runs in the fused gate + norm kernel."""
+
+    def __init__(self, d):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(d))
+
+
+class LinearAttention(StateLifecycle, nn.Module):
+    """Mixer: x -> [one GEMM: q | k | v | gate z] -> `linear_attention` -> y * silu(z) (+ RMSNorm) -> out_proj.
+
+    ``LinearAttention(config, execution=None)``; same call, `State` and `step` contract as the package's other mixers, so it
+    stands in `ResidualBlock`, `BlockStack`, `GraphedStep` and `GraphedDecode` beside them."""
+
+    config_family = "linear_attention"
+    fused_residual = True
+
+    def __init__(self, config, execution=None):
+        nn.Module.__init__(self)
+        if isinstance(config, dict):
+            config = LinearAttentionConfig.from_dict(config)
+        if not isinstance(config, LinearAttentionConfig):
+            raise TypeError(f"config must be a LinearAttentionConfig or its dict, got {type(config).__name__}")
+        self.config = c = config
+        self.d_model, self.H, self.Dk, self.Dv = c.d_model, c.n_heads, c.d_key, c.d_value
+        dk, dv = self.H * self.Dk, self.H * self.Dv
+        self.q_proj = nn.Linear(c.d_model, dk, bias=False)
+        self.k_proj = nn.Linear(c.d_model, dk, bias=False)
+        self.v_proj = nn.Linear(c.d_model, dv, bias=False)
+        self.gate_proj = nn.Linear(c.d_model, dv, bias=False)
+        spans = torch.logspace(math.log2(c.span_min), math.log2(c.span_max), self.H, base=2.0, dtype=torch.float64)
+        self.register_buffer("log_decay", torch.log1p(-1.0 / spans).float(), persistent=True)
+        self.norm = _OutNorm(dv) if c.out_norm else nn.Identity()
+        self.out_proj = nn.Linear(dv, c.d_model, bias=False)
+        # the columns of a bfloat16 slab stay 16-byte aligned for any head widths that the tensor-core tiles take
+        self._pad = (-(2 * dk + 2 * dv)) % 8
+        self.backend, self.precision, self.chunk_size, self.kernel_options = "cuda", "io", "auto", {}
+        self._final_state = None
+        self.set_execution(as_execution(execution))
+
+    # -- execution ------------------------------------------------------------------------------------------
+    def _check_execution(self, ex):
+        f, out = ex.fields(), {}
+        if "backend" in f:
+            if f["backend"] not in BACKENDS:
+                raise ValueError(f"LinearAttention: backend must be one of {BACKENDS}, got {f['backend']!r}")
+            out["backend"] = f["backend"]
+        if "precision" in f:
+            if f["precision"] not in PRECISIONS:
+                raise ValueError(f"LinearAttention: precision must be one of {PRECISIONS}, got {f['precision']!r}")
+            if f["precision"] != "io":
+                raise ValueError("LinearAttention: precision='ieee' is refused: the kernels go by the activations' dtype (float32 "
+                                 "activations run in float32)")
+        if "chunk_size" in f and f["chunk_size"] != "auto":
+            raise ValueError(f"LinearAttention: chunk_size is the kernels' own ('auto'), got {f['chunk_size']!r}")
+        if f.get("checkpoint"):
+            raise ValueError("LinearAttention: checkpoint=True is refused (BlockStack.set_checkpoint keeps block inputs in 8 bits)")
+        if f.get("kernel_options"):
+            raise ValueError(f"LinearAttention: unknown kernel option(s) {sorted(f['kernel_options'])}; this layer has none")
+        return out
+
+    def set_execution(self, execution):
+        for k, v in self._check_execution(as_execution(execution)).items():
+            setattr(self, k, v)
+        return self
+
+    # -- state ----------------------------------------------------------------------------------------------
+    def _init_state(self, batch_size, device=None, dtype=None):
+        dev = device if device is not None else next(self.parameters()).device
+        return State(hidden_state=torch.zeros(batch_size, self.H, self.Dv, self.Dk, device=dev,
+                                              dtype=self._default_state_dtype() if dtype is None else dtype))
+
+    def hidden_state_shape(self):
+        return (self.H, self.Dv, self.Dk)
+
+    # -- forward --------------------------------------------------------------------------------------------
+    def forward(self, x, *, state=None, return_state=False, _residual=None):
+        """x [B, L, d_model] -> y [B, L, d_model], or (y, State) with ``return_state=True``; `state` continues a previous call."""
+        if x.dim() != 3 or x.shape[-1] != self.d_model:
+            raise ValueError(f"LinearAttention: expected x of shape [B, L, {self.d_model}], got {tuple(x.shape)}")
+        if not ops.on_device(x):
+            raise ValueError("LinearAttention: got a CPU tensor; this layer runs on a CUDA device only")
+        B, L, _ = x.shape
+        H, Dk, Dv = self.H, self.Dk, self.Dv
+        if state is not None:
+            state = self.resolve_state(state, batch_size=B, device=x.device)
+        io = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+        if io not in (torch.float32, torch.bfloat16):
+            raise NotImplementedError(f"LinearAttention: IO dtype must be float32 or bfloat16, got {io}")
+        with torch.autocast("cuda", enabled=False):
+            proj = ops.ProjectFn.apply(x.to(io), None, self._pad, None, 0, self.q_proj.weight, self.k_proj.weight, self.v_proj.weight,
+                                       self.gate_proj.weight)
+            arena = ops.GradArena()                  # the operators' backward passes write d(proj) in place
+            q, k, v, z = ops.SplitColumnsFn.apply(proj, arena, H * Dk, H * Dk, H * Dv, H * Dv)
+            q, k, v = q.unflatten(2, (H, Dk)), k.unflatten(2, (H, Dk)), v.unflatten(2, (H, Dv))
+            s0 = None if state is None else state["hidden_state"].to(torch.float32)
+            if L == 1 and s0 is not None and not torch.is_grad_enabled():
+                y, new = linear_attention_step(q[:, 0], k[:, 0], v[:, 0], self.log_decay, s0)
+                y = y.unsqueeze(1)
+            else:
+                y = linear_attention(q, k, v, self.log_decay, s0, return_state=return_state,
+                                     _slots=((arena, 0), (arena, 1), (arena, 2)))
+                y, new = y if return_state else (y, None)
+            y = y.flatten(2)
+            if L > 0:
+                y = ops.GateNormFn.apply(y, z, self.norm.weight if self.config.out_norm else None, self.config.norm_eps, (arena, 3))
+            fuse = _residual is not None and _residual.dtype == io and _residual.shape == x.shape
+            out = ops.ProjectFn.apply(y, _residual if fuse else None, 0, None, 0, self.out_proj.weight)
+            if _residual is not None and not fuse:
+                out = _residual + out
+        if not return_state:
+            return out
+        ordered = self._conform_carries(State(hidden_state=new), state)
+        self._final_state = ordered
+        return out, ordered
+
+    def step(self, x_t, state=None):
+        """One token: ``x_t [B, d_model]``, `state` from `init_state` or a previous call -> ``(y_t [B, d_model], State)``.  Under
+        ``torch.no_grad()`` the token runs in the one-launch step kernel; with gradients it is a sequence of one token."""
+        if x_t.dim() != 2 or x_t.shape[-1] != self.d_model:
+            raise ValueError(f"LinearAttention.step: expected x_t of shape [B, {self.d_model}], got {tuple(x_t.shape)}")
+        if state is None:
+            state = self.init_state(x_t.shape[0], device=x_t.device)
+        y, new = self.forward(x_t.unsqueeze(1), state=state, return_state=True)
+        return y.squeeze(1), new
