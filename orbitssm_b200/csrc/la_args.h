@@ -28,7 +28,7 @@ struct LaJob {
 };
 struct LaPlan {
   int B, L, H, S;     // S = Dk * Dv, elements of a head's state
-  int njobs, nseg, seg_len;
+  int njobs, nseg, seg_len, ne;   // ne: tiles of output channels (tensor-core launch)
   const float* log_decay;
   int* status;
   LaJob job[3];
