@@ -3,22 +3,26 @@
 // is 128 tokens and its products are tensor-core tiles with float32 accumulators in TMEM.
 //
 // One CTA owns (batch, head, segment, 64 channels of v') and walks the chunks of its segment:
-//   S1[t,s] = q'_t . k'_s                    128 x 128 x X     both operands as TMA wrote them
-//   P       = decay mask o S1 -> bfloat16                      the only rounding of the part inside the chunk
-//   O [t,e] = P V'                           128 x 64 x 128    P read from TMEM
-//   O2[t,e] = q'_t . Zb                      128 x 64 x X      Zb: the state rounded to bfloat16, the only rounding of that part
-//   dZ[x,e] = sum_s k'_s[x] (f_s v'_s[e])    128 x 192 x 128   f_s v' in three bfloat16 parts (hi + mid + lo hold all 24 bits of
+//   S1[t,s] = q'_t . k'_s                      128 x 128 x X   both operands as TMA wrote them
+//   P[t,s]  = S1[t,s] a^{c-s} (s <= t, else 0) -> bfloat16     the only rounding of the part inside the chunk
+//   O[t,e]  = P v' + q' Zb                     128 x 64 x (128 + X)   P read from TMEM; Zb = a^{c+1} s_in / s_out Z rounded to
+//                                                              bfloat16, the only rounding of that part
+//   dZ[x,e] = sum_s k'_s[x] (f_s v'_s[e])      128 x 192 x 128 f_s v' in three bfloat16 parts (hi + mid + lo hold all 24 bits of
 //                                                              the float32 product) side by side, so that the float32 state and
 //                                                              the state's gradient lose nothing to the operands' type
-//   out = s_out O + s_in a^{..} O2;   Z = a^T Z + dZ           Z in registers, float32
-// Row factors are applied to the accumulators, not to the operands: scaling q' or k' first would round them once more.
+//   out = s_out a^{t-c} O;   Z = a^T Z + dZ                    Z in registers, float32
+// The decay a^{t-s} is split into a column factor on the scores and a row factor on the float32 accumulator, counted from the
+// middle of the chunk (c = 64; backwards in time a^{s-c} and a^{c-t}, c = 63), so that both parts of the output meet in one
+// accumulator and no operand is rounded twice.  That needs a^{-64} to stay far from overflow: heads with a < 1/2 (`steep`) keep
+// a^{t-s} on the scores, where it is at most 1, and the two parts in accumulators of their own.
 //
-// Warp-specialised, 18 warps that meet only through mbarriers (every wait bounded):
-//   warps 0..3   decay mask: S1 -> P (TMEM to TMEM; the slabs beyond the diagonal are zero and written once)
-//   warps 4..7   state: Z in registers (thread = state row), writes Zb, adds dZ
-//   warps 8..11  scaled v': three bfloat16 tiles (thread = token)
-//   warps 12..15 read-out: O, O2 -> output tile in the place of the v' tile -> TMA store
-//   warp 16      one lane issues the TMA loads (two stages), warp 17 one lane issues the MMAs
+// Warp-specialised, 27 warps that meet only through mbarriers (every wait bounded):
+//   warps 0..3   decay mask: S1 -> P (TMEM to TMEM; the 32-column slabs beyond the diagonal are zero and written once)
+//   warps 4..11  state: Z in registers (thread = state row, 32 of its channels), writes Zb, adds dZ
+//   warps 12..19 scaled v': three bfloat16 tiles (thread = token, 32 channels)
+//   warps 20..23 read-out: O -> output tile in the place of the v' tile -> TMA store
+//   warp 24      one lane issues the TMA loads (two stages); warp 25 the MMAs S1 and O, warp 26 those of dZ
+// Two issuing warps: the tensor pipe then has work of one queue while the other waits for its operands.
 // 64 channels a CTA (two CTAs for a 128-wide head, adjacent so that q' and k' come from L2 the second time): the state then
 // leaves room in shared memory for two stages of operands, and short batches fill twice the SMs.
 #include "common.cuh"
@@ -29,10 +33,13 @@
 namespace orbit {
 using namespace tc;
 
-constexpr int LT_T = 128, LT_E = 64, LT_THREADS = 576;
-constexpr uint32_t LT_S1 = 0, LT_P = 128, LT_O = 192, LT_O2 = 256, LT_DZ = 320;   // TMEM columns (512 in all)
+constexpr int LT_T = 128, LT_E = 64;
+constexpr int LT_ZG = 2, LT_VG = 2;   // groups of four warps for the state and for v'
+constexpr int LT_W_V = 4 + 4 * LT_ZG, LT_W_OUT = LT_W_V + 4 * LT_VG, LT_W_LOAD = LT_W_OUT + 4, LT_THREADS = (LT_W_LOAD + 3) * 32;   // first warps of the roles
+constexpr uint32_t LT_S1 = 0, LT_P = 128, LT_O = 192, LT_DZ = 320;   // TMEM columns: 128, 64, 2 x 64, 192 (512 in all)
 constexpr int LT_STAGE = 5;                                  // blocks of 16 KB: q' 2, k' 2, v' 1
 constexpr int LT_SMEM = (2 * LT_STAGE + 3 + 1) * (int)BLK + 1024;
+constexpr int LT_FWD_C = 64, LT_REV_C = 63;                  // the token that decays are counted from
 
 struct LaTcArgs {
   CUtensorMap map[3][4];                                     // q', k', v', output of each job
@@ -40,8 +47,8 @@ struct LaTcArgs {
 };
 
 struct LtBars {
-  uint64_t qk_full[2], qk_empty[2], v_full[2], v_empty[2], s1_full, s1_empty, p_full, p_empty, vd_full, vd_empty, zb_full,
-      zb_empty, dz_full, dz_empty, acc_full, acc_empty;
+  uint64_t qk_full[2], qk_empty[2], v_full[2], v_empty[2], v_read[2], s1_full, s1_empty, p_full, p_empty, vd_full, vd_empty, zb_full,
+      zb_empty, dz_full, dz_empty, acc_full[2], acc_empty[2];
 };
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z, int w) {
@@ -57,71 +64,81 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, const void* s
                "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
-__device__ __forceinline__ float bf16_round(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+// a^n for |n| <= 128 from the table of a^0 .. a^128 (n < 0 only where a is at least 1/2)
+__device__ __forceinline__ float power(const float* pw, int n) { return n >= 0 ? pw[n] : __fdividef(1.f, pw[-n]); }
 
-__global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_constant__ LaTcArgs a, const int local) {
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ LtBars bars;
-  __shared__ float pw[LT_T + 1];                             // a^0 .. a^128
-  __shared__ uint32_t tmem_slot;
-  __shared__ int s_abort;
+// One lane of a converged warp, the same one every time.  Issued under a plain `lane == 0` test the compiler takes the MMA's
+// operands for values that differ between lanes: 94 cycles an instruction at N = 64 against 75, and 94 against 42 with the
+// operand in TMEM (measured alone; the four products of a chunk 4450 cycles against 2000).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+
+struct LtShared {
+  LtBars bars;
+  float pw[LT_T + 1];                                        // a^0 .. a^128
+  uint32_t tmem_slot;
+  int abort_flag;
+};
+
+// The walk of one CTA; the compiler's copies for each direction, kind of head and launch keep the loops of the roles short.
+template <bool rev, bool steep, bool local>
+__device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint8_t* sm, const int jb, const int b, const int h,
+                                           const int seg, const int et, const double ld) {
   const LaPlan& p = a.p;
-  // tile index: e tile fastest, then job, segment, head, batch
-  int64_t id = blockIdx.x;
-  const int ne = p.ne;
-  const int et = (int)(id % ne);
-  id /= ne;
-  const int jb = (int)(id % p.njobs);
-  id /= p.njobs;
-  const int seg = (int)(id % p.nseg);
-  id /= p.nseg;
-  const int h = (int)(id % p.H), b = (int)(id / p.H), e0 = et * LT_E;
   const LaJob& J = p.job[jb];
-  const int rev = J.reverse, X = J.X, E = J.E;
-  if (e0 >= E) return;
-  if (local && seg == (rev ? 0 : p.nseg - 1)) return;        // nobody reads the last segment's share
+  const int X = J.X, E = J.E, e0 = et * LT_E;
   const CUtensorMap *mq = &a.map[jb][0], *mk = &a.map[jb][1], *mv = &a.map[jb][2], *my = &a.map[jb][3];
-
-  uint8_t* sm = align1024(smem_raw);
+  LtBars& bars = sh.bars;
+  const float* pw = sh.pw;
   uint8_t* sVd = sm + 2 * LT_STAGE * BLK;                    // scaled v': hi, mid, lo
   uint8_t* sZb = sVd + 3 * BLK;                              // entering state, bfloat16 [128 x][64 e]
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, role = warp >> 2;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3;
   const int s0 = seg * p.seg_len, s1 = min(p.L, s0 + p.seg_len), nch = (s1 - s0 + LT_T - 1) / LT_T;
-  const double ld = (double)p.log_decay[h];
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.qk_full[i], 1);
-      mbar_init(&bars.qk_empty[i], 1);
+      mbar_init(&bars.qk_empty[i], local ? 1 : 2);           // released by both issuing warps
       mbar_init(&bars.v_full[i], 1);
-      mbar_init(&bars.v_empty[i], 1);
+      mbar_init(&bars.v_empty[i], local ? 4 * LT_VG : 1);    // by the read-out, which puts its tile there (local: the scaling warps)
+      mbar_init(&bars.v_read[i], 4 * LT_VG);
+      mbar_init(&bars.acc_full[i], 1);
+      mbar_init(&bars.acc_empty[i], 4);
     }
     mbar_init(&bars.s1_full, 1);
     mbar_init(&bars.s1_empty, 4);
     mbar_init(&bars.p_full, 4);
     mbar_init(&bars.p_empty, 1);
-    mbar_init(&bars.vd_full, 4);
+    mbar_init(&bars.vd_full, 4 * LT_VG);
     mbar_init(&bars.vd_empty, 1);
-    mbar_init(&bars.zb_full, 4);
+    mbar_init(&bars.zb_full, 4 * LT_ZG);
     mbar_init(&bars.zb_empty, 1);
     mbar_init(&bars.dz_full, 1);
-    mbar_init(&bars.dz_empty, 4);
-    mbar_init(&bars.acc_full, 1);
-    mbar_init(&bars.acc_empty, 4);
+    mbar_init(&bars.dz_empty, 4 * LT_ZG);
     mbar_fence_init();
-    s_abort = 0;
+    sh.abort_flag = 0;
   }
-  if (tid <= LT_T) pw[tid] = tid == 0 ? 1.f : (float)exp(ld * tid);
-  if (warp == 0) tmem_alloc(&tmem_slot, 512);
+  if (tid <= LT_T) sh.pw[tid] = tid == 0 ? 1.f : (float)exp(ld * tid);
+  if (warp == 0) tmem_alloc(&sh.tmem_slot, 512);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tbase = tmem_slot;
-  volatile int* abort_flag = &s_abort;
+  const uint32_t tbase = sh.tmem_slot;
+  volatile int* abort_flag = &sh.abort_flag;
   bool dead = false;
+  // The state is kept times the factor that makes the carried part share the row factor of the other (steep heads and the
+  // state-only launch: as it is), so that Zb is one rounding of what the registers hold.
+  const float zscale = steep || local ? 1.f : J.s_in / J.s_out * power(pw, rev ? LT_T - 1 - LT_REV_C : LT_FWD_C + 1);
   auto chunk_start = [&](int c) { return s0 + (rev ? nch - 1 - c : c) * LT_T; };
 
-  if (warp == 16) {
+  if (warp == LT_W_LOAD) {
     if (lane == 0) {
       // ---- producer ----
       int done = 0;
@@ -148,108 +165,140 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       }
     }
     __syncwarp();
-  } else if (warp == 17) {
-    if (lane == 0) {
-      // ---- MMA issuer ----
-      const uint32_t id_s = idesc_bf16(128, 128, 0, 0), id_o = idesc_bf16(128, 64, 0, 1), id_z = idesc_bf16(128, 192, 1, 1);
+  } else if (warp == LT_W_LOAD + 1) {
+    // ---- MMA issuer of the scores and the output: the warp waits, one lane issues ----
+    if (!local) {
+      const uint32_t id_s = idesc_bf16(128, 128, 0, 0), id_o = idesc_bf16(128, 64, 0, 1);
       const int kx = (X + 15) / 16;
-      const uint32_t vd = lo_mn(smem_u32(sVd)), zb = lo_mn(smem_u32(sZb));
+      const uint32_t zb = lo_mn(smem_u32(sZb));
       auto base = [&](int c, int blk) { return smem_u32(sm + ((c & 1) * LT_STAGE + blk) * BLK); };
       auto scores = [&](int c) {
         const uint32_t aq = lo_k(base(c, 0)), bk = lo_k(base(c, 2));
+        if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
-          if (ks < kx) umma_bf16_h(tbase + LT_S1, aq + inc_k(ks), bk + inc_k(ks), id_s, ks > 0 ? 1u : 0u);
-        umma_commit(&bars.s1_full);
+          for (int ks = 0; ks < 8; ++ks)
+            if (ks < kx) umma_bf16_h(tbase + LT_S1, aq + inc_k(ks), bk + inc_k(ks), id_s, ks > 0 ? 1u : 0u);
+          umma_commit(&bars.s1_full);
+        }
       };
-      if (lane_wait(&bars.qk_full[0], 0, abort_flag, dead) && !local) {
+      if (role_wait(&bars.qk_full[0], 0, abort_flag, dead)) {
         tc_fence_after_sync();
         scores(0);
       }
 #pragma unroll 1
       for (int c = 0; c < nch && !dead; ++c) {
-        const uint32_t ph = (uint32_t)(c & 1), prev = (uint32_t)((c - 1) & 1);
-        if (local && c > 0 && !lane_wait(&bars.qk_full[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead)) break;
-        if (!local) {
-          if (!lane_wait(&bars.zb_full, ph, abort_flag, dead)) break;
-          if (c > 0 && !lane_wait(&bars.acc_empty, prev, abort_flag, dead)) break;
-          tc_fence_after_sync();
-          const uint32_t aq = lo_k(base(c, 0));
+        const uint32_t ph = (uint32_t)(c & 1);
+        // accumulators of this chunk: one of two sets; steep heads use both, for the two parts
+        const uint32_t acc2 = tbase + LT_O + (steep ? 0u : ph * 64u), acc1 = steep ? tbase + LT_O + 64u : acc2;
+        if (!role_wait(&bars.zb_full, ph, abort_flag, dead)) break;
+        if (steep && c > 0 && !role_wait(&bars.acc_empty[ph ^ 1u], (uint32_t)(((c - 1) >> 1) & 1), abort_flag, dead)) break;
+        if (!steep && c > 1 && !role_wait(&bars.acc_empty[ph], (uint32_t)(((c >> 1) - 1) & 1), abort_flag, dead)) break;
+        tc_fence_after_sync();
+        const uint32_t aq = lo_k(base(c, 0));
+        if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
-            if (ks < kx) umma_bf16_h(tbase + LT_O2, aq + inc_k(ks), zb + inc_mn(ks), id_o, ks > 0 ? 1u : 0u);
+            if (ks < kx) umma_bf16_h(acc2, aq + inc_k(ks), zb + inc_mn(ks), id_o, ks > 0 ? 1u : 0u);
           umma_commit(&bars.zb_empty);
+          umma_commit(&bars.qk_empty[c & 1]);                // this warp has read q' and k' of the chunk for the last time
         }
-        if (!lane_wait(&bars.vd_full, ph, abort_flag, dead)) break;
-        if (c > 0 && !lane_wait(&bars.dz_empty, prev, abort_flag, dead)) break;
+        if (c + 1 < nch) {
+          if (!role_wait(&bars.qk_full[(c + 1) & 1], (uint32_t)(((c + 1) >> 1) & 1), abort_flag, dead)) break;
+          if (!role_wait(&bars.s1_empty, ph, abort_flag, dead)) break;
+          tc_fence_after_sync();
+          scores(c + 1);
+        }
+        if (!role_wait(&bars.p_full, ph, abort_flag, dead)) break;
+        if (!role_wait(&bars.v_full[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead)) break;
         tc_fence_after_sync();
-        const uint32_t ak = lo_mn(base(c, 2));
+        const uint32_t bv = lo_mn(base(c, 4));
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)
+            umma_bf16_ta_h(acc1, tbase + LT_P + ks * 8, bv + inc_mn(ks), id_o, (ks > 0 || !steep) ? 1u : 0u);
+          umma_commit(&bars.p_empty);
+          umma_commit(&bars.acc_full[c & 1]);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == LT_W_LOAD + 2) {
+    // ---- MMA issuer of the state update ----
+    const uint32_t id_z = idesc_bf16(128, 192, 1, 1), vd = lo_mn(smem_u32(sVd));
+#pragma unroll 1
+    for (int c = 0; c < nch && !dead; ++c) {
+      if (!role_wait(&bars.qk_full[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead)) break;
+      if (c > 0 && !role_wait(&bars.dz_empty, (uint32_t)((c - 1) & 1), abort_flag, dead)) break;
+      if (!role_wait(&bars.vd_full, (uint32_t)(c & 1), abort_flag, dead)) break;
+      tc_fence_after_sync();
+      const uint32_t ak = lo_mn(smem_u32(sm + ((c & 1) * LT_STAGE + 2) * BLK));
+      if (elect_one()) {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) umma_bf16_h(tbase + LT_DZ, ak + inc_mn(ks), vd + inc_mn(ks), id_z, ks > 0 ? 1u : 0u);
         umma_commit(&bars.dz_full);
         umma_commit(&bars.vd_empty);
-        umma_commit(&bars.qk_empty[c & 1]);                  // q' and k' of this chunk have been read for the last time
-        if (local) continue;
-        if (c + 1 < nch) {
-          if (!lane_wait(&bars.qk_full[(c + 1) & 1], (uint32_t)(((c + 1) >> 1) & 1), abort_flag, dead)) break;
-          if (!lane_wait(&bars.s1_empty, ph, abort_flag, dead)) break;
-          tc_fence_after_sync();
-          scores(c + 1);
-        }
-        if (!lane_wait(&bars.p_full, ph, abort_flag, dead)) break;
-        tc_fence_after_sync();
-        const uint32_t bv = lo_mn(base(c, 4));
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
-          umma_bf16_ta_h(tbase + LT_O, tbase + LT_P + ks * 8, bv + inc_mn(ks), id_o, ks > 0 ? 1u : 0u);
-        umma_commit(&bars.p_empty);
-        umma_commit(&bars.acc_full);
+        umma_commit(&bars.qk_empty[c & 1]);
       }
     }
     __syncwarp();
-  } else if (role == 0) {
+  } else if (warp < 4) {
     if (!local) {
       // ---- decay mask: thread = row t; slab j holds columns 32 j .. 32 j + 31 ----
       {
         uint32_t z[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) z[i] = 0u;
-#pragma unroll
+#pragma unroll 1
         for (int j = 0; j < 4; ++j)
           if (rev ? j < q : j > q) tmem_st16(tmem_addr(tbase, q * 32, LT_P + j * 16), z);
         tmem_st_wait();
       }
+      const int j0 = rev ? q : 0, j1 = rev ? 3 : q;
+      // Column factors a^{c-s} (reverse a^{s-c}) run along the row by repeated multiplication, two chains of pairs: at most 32
+      // products of rounded factors, off by 2^-18, against the 2^-8 of the rounding that follows.  Shared memory is busy with the
+      // MMAs' operands: a table there costs its latency for every few elements.
+      const int n0 = rev ? 32 * q - LT_REV_C : LT_FWD_C, d0 = rev ? 1 : -1;
+      const float a4 = steep ? 0.f : power(pw, 4 * d0);
+      const float2 step = make_float2(a4, a4);
+      const float2 g0 = steep ? step : make_float2(power(pw, n0), power(pw, n0 + d0));
+      const float2 g1 = steep ? step : make_float2(power(pw, n0 + 2 * d0), power(pw, n0 + 3 * d0));
 #pragma unroll 1
       for (int c = 0; c < nch; ++c) {
         bool ok = role_wait(&bars.s1_full, (uint32_t)(c & 1), abort_flag, dead);
         if (c > 0) ok = role_wait(&bars.p_empty, (uint32_t)((c - 1) & 1), abort_flag, dead) && ok;
         if (ok) {
           tc_fence_after_sync();
+          float2 f0 = g0, f1 = g1;
 #pragma unroll 1
-          for (int j = rev ? q : 0; j <= (rev ? 3 : q); ++j) {
+          for (int j = j0; j <= j1; ++j) {
             uint32_t r[32], o[16];
             tmem_ld32(tmem_addr(tbase, q * 32, LT_S1 + j * 32), r);
             tmem_ld_wait();
-            if (j == q) {
-              // a^{t-s} on and below the diagonal (reverse: a^{s-t} on and above it); zero beyond, whatever the score
+            if (!steep) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int d0 = rev ? 2 * i - lane : lane - 2 * i, d1 = rev ? 2 * i + 1 - lane : lane - 2 * i - 1;
-                const float f0 = pw[max(d0, 0)], f1 = pw[max(d1, 0)];
-                o[i] = pack_bf16(d0 >= 0 ? __uint_as_float(r[2 * i]) * f0 : 0.f, d1 >= 0 ? __uint_as_float(r[2 * i + 1]) * f1 : 0.f);
+              for (int i = 0; i < 8; ++i) {
+                const float2 u = mul2(f2(r[4 * i], r[4 * i + 1]), f0), w = mul2(f2(r[4 * i + 2], r[4 * i + 3]), f1);
+                f0 = mul2(f0, step);
+                f1 = mul2(f1, step);
+                r[4 * i] = __float_as_uint(u.x);
+                r[4 * i + 1] = __float_as_uint(u.y);
+                r[4 * i + 2] = __float_as_uint(w.x);
+                r[4 * i + 3] = __float_as_uint(w.y);
               }
             } else {
-              // a whole slab away the factor splits at the slab's near end: both parts are powers of a that are at least one
-              // factor each, so neither grows beyond 1
-              const float rf = pw[rev ? 32 * (j - q) - lane : 32 * (q - j) + lane - 31];
-              const float2 rf2 = make_float2(rf, rf);
+              // a^{t-s} from the powers themselves: at most 1 wherever the score is kept
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 cf = rev ? make_float2(pw[2 * i], pw[2 * i + 1]) : make_float2(pw[31 - 2 * i], pw[30 - 2 * i]);
-                const float2 v = mul2(f2(r[2 * i], r[2 * i + 1]), mul2(rf2, cf));
-                o[i] = pack_bf16(v.x, v.y);
+              for (int i = 0; i < 32; ++i) {
+                const int n = rev ? 32 * (j - q) + i - lane : 32 * (q - j) + lane - i;
+                r[i] = __float_as_uint(__uint_as_float(r[i]) * pw[max(n, 0)]);
               }
             }
+            if (j == q) {                                    // zero beyond the diagonal, whatever the score
+#pragma unroll
+              for (int i = 0; i < 32; ++i) r[i] = (rev ? i >= lane : i <= lane) ? r[i] : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = pack_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
             tmem_st16(tmem_addr(tbase, q * 32, LT_P + j * 16), o);
           }
           tmem_st_wait();
@@ -258,21 +307,23 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         if (lane == 0) mbar_arrive(&bars.p_full);
       }
     }
-  } else if (role == 1) {
-    // ---- state: thread = state row x, its 64 channels in registers ----
+  } else if (warp < LT_W_V) {
+    // ---- state: thread = state row x, ZE of its channels in registers ----
+    constexpr int ZE = LT_E / LT_ZG;
+    const int hf = (warp - 4) >> 2, ez = hf * ZE;            // first of this thread's channels in the tile
     const int x = q * 32 + lane;
     const int64_t head = (int64_t)b * p.H + h;
-    float z[LT_E];
+    float z[ZE];
 #pragma unroll
-    for (int e = 0; e < LT_E; ++e) z[e] = 0.f;
+    for (int e = 0; e < ZE; ++e) z[e] = 0.f;
     const bool live = x < X;
     if (!local && live) {
       // the carried state and the shares of the segments before this one, each with its decay since
-      const int64_t off = x * J.xs + e0 * J.es;
+      const int64_t off = x * J.xs + (e0 + ez) * J.es;
       if (J.z0) {
         const float* src = J.z0 + head * p.S + off;
 #pragma unroll
-        for (int e = 0; e < LT_E; ++e) if (e0 + e < E) z[e] = src[e * J.es];
+        for (int e = 0; e < ZE; ++e) if (e0 + ez + e < E) z[e] = src[e * J.es];
       }
       if (J.part) {
         const float full = (float)exp(ld * p.seg_len);
@@ -283,119 +334,163 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
           const float f = s == p.nseg - 1 ? (float)exp(ld * (p.L - s * p.seg_len)) : full;
           const float* src = J.part + (head * p.nseg + s) * p.S + off;
 #pragma unroll
-          for (int e = 0; e < LT_E; ++e) if (e0 + e < E) z[e] = fmaf(f, z[e], src[e * J.es]);
+          for (int e = 0; e < ZE; ++e) if (e0 + ez + e < E) z[e] = fmaf(f, z[e], src[e * J.es]);
         }
       }
     }
+    if (!local) {
+#pragma unroll
+      for (int e = 0; e < ZE; ++e) z[e] *= zscale;
+    }
+    const float a_full = pw[LT_T];
 #pragma unroll 1
     for (int c = 0; c < nch; ++c) {
+      const int Tv = min(LT_T, s1 - chunk_start(c));
       if (!local) {
         bool ok = !dead;
         if (c > 0) ok = role_wait(&bars.zb_empty, (uint32_t)((c - 1) & 1), abort_flag, dead);
         if (ok) {
+          const bool odd = rev && !steep && Tv != LT_T;      // a ragged chunk is counted from its own end backwards in time
+          const float zs = odd ? __fdividef(1.f, pw[LT_T - Tv]) : 1.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(sZb + sw128_offset(x, j)) =
-                make_uint4(pack_bf16(z[8 * j], z[8 * j + 1]), pack_bf16(z[8 * j + 2], z[8 * j + 3]), pack_bf16(z[8 * j + 4], z[8 * j + 5]),
-                           pack_bf16(z[8 * j + 6], z[8 * j + 7]));
+          for (int j = 0; j < ZE / 8; ++j) {
+            float2 y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              y[i] = make_float2(z[8 * j + 2 * i], z[8 * j + 2 * i + 1]);
+              if (odd) y[i] = mul2(y[i], make_float2(zs, zs));
+            }
+            *reinterpret_cast<uint4*>(sZb + sw128_offset(x, ez / 8 + j)) =
+                make_uint4(pack_bf16(y[0].x, y[0].y), pack_bf16(y[1].x, y[1].y), pack_bf16(y[2].x, y[2].y), pack_bf16(y[3].x, y[3].y));
+          }
         }
         warp_arrive(&bars.zb_full, true);
       }
-      const float aT = pw[min(LT_T, s1 - chunk_start(c))];
+      const float aT = Tv == LT_T ? a_full : pw[Tv];
       if (role_wait(&bars.dz_full, (uint32_t)(c & 1), abort_flag, dead)) {
         tc_fence_after_sync();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < ZE / 8; ++j) {
           uint32_t hi[8], mi[8], lo[8];
-          tmem_ld8(tmem_addr(tbase, q * 32, LT_DZ + j * 8), hi);
-          tmem_ld8(tmem_addr(tbase, q * 32, LT_DZ + 64 + j * 8), mi);
-          tmem_ld8(tmem_addr(tbase, q * 32, LT_DZ + 128 + j * 8), lo);
+          tmem_ld8(tmem_addr(tbase, q * 32, LT_DZ + ez + j * 8), hi);
+          tmem_ld8(tmem_addr(tbase, q * 32, LT_DZ + 64 + ez + j * 8), mi);
+          tmem_ld8(tmem_addr(tbase, q * 32, LT_DZ + 128 + ez + j * 8), lo);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            z[8 * j + i] = fmaf(aT, z[8 * j + i], __uint_as_float(hi[i]) + (__uint_as_float(mi[i]) + __uint_as_float(lo[i])));
+          for (int i = 0; i < 8; i += 2) {
+            const float2 d = add2(f2(hi[i], hi[i + 1]), add2(f2(mi[i], mi[i + 1]), f2(lo[i], lo[i + 1])));
+            const float2 y = fma2(make_float2(aT, aT), make_float2(z[8 * j + i], z[8 * j + i + 1]), d);
+            z[8 * j + i] = y.x;
+            z[8 * j + i + 1] = y.y;
+          }
         }
       }
       warp_arrive(&bars.dz_empty, false);
     }
     float* out = local ? J.part + (head * p.nseg + seg) * p.S : (J.z1 && seg == (rev ? 0 : p.nseg - 1) ? J.z1 + head * p.S : nullptr);
     if (out && live && !dead) {
-      out += x * J.xs + e0 * J.es;
+      out += x * J.xs + (e0 + ez) * J.es;
+      const float unscale = 1.f / zscale;
 #pragma unroll
-      for (int e = 0; e < LT_E; ++e) if (e0 + e < E) out[e * J.es] = z[e];
+      for (int e = 0; e < ZE; ++e) if (e0 + ez + e < E) out[e * J.es] = z[e] * unscale;
     }
-  } else if (role == 2) {
-    // ---- scaled v': thread = token s; f v = hi + mid + lo exactly (each difference is exact in float32) ----
-    const int s = q * 32 + lane;
+  } else if (warp < LT_W_OUT) {
+    // ---- scaled v': thread = token s, all in packed bfloat16 arithmetic (fma with one rounding): with the factor
+    // f = f1 + f2 + f3 in bfloat16 parts (24 bits),
+    //   hi = rn(v f1),  m = v f1 - hi (exact),  mid = rn(v f2 + m),  lo = rn(rn(v f2 + (m - mid)) + v f3)
+    // and hi + mid + lo is f v to 2^-23 of it.  Six instructions a pair; splitting the float32 product takes twelve. ----
+    constexpr int VJ = 8 / LT_VG;                            // 16-byte pieces of a row
+    const int s = q * 32 + lane, j0 = ((warp - LT_W_V) >> 2) * VJ;
+    auto split = [&](float f, __nv_bfloat162(&fp)[3]) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const __nv_bfloat16 part = __float2bfloat16_rn(f);
+        fp[i] = __nv_bfloat162(part, part);
+        f -= __bfloat162float(part);
+      }
+    };
+    const float fz = local ? J.s_state : J.s_state * zscale;
+    __nv_bfloat162 full[3];
+    split(fz * pw[rev ? s + 1 : LT_T - 1 - s], full);
+    const uint32_t row = s * 128u, sw = s & 7u;
 #pragma unroll 1
     for (int c = 0; c < nch; ++c) {
       const int Tv = min(LT_T, s1 - chunk_start(c));
-      const float f = s < Tv ? J.s_state * pw[rev ? s + 1 : Tv - 1 - s] : 0.f;
+      __nv_bfloat162 f[3] = {full[0], full[1], full[2]};
+      if (Tv != LT_T) split(s < Tv ? fz * pw[rev ? s + 1 : Tv - 1 - s] : 0.f, f);
       const uint8_t* v = sm + ((c & 1) * LT_STAGE + 4) * BLK;
+      uint4 w[VJ];
       bool ok = role_wait(&bars.v_full[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead);
+      if (ok) {
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) w[j] = *reinterpret_cast<const uint4*>(v + row + (((j0 + j) ^ sw) << 4));   // all of them before the first store
+      }
       if (c > 0) ok = role_wait(&bars.vd_empty, (uint32_t)((c - 1) & 1), abort_flag, dead) && ok;
       if (ok) {
-#pragma unroll 2
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t off = sw128_offset(s, j);
-          const uint4 w = *reinterpret_cast<const uint4*>(v + off);
-          const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-          uint32_t oh[4], om[4], ol[4];
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) {
+          uint4 oh, om, ol;
+          const __nv_bfloat162* in = reinterpret_cast<const __nv_bfloat162*>(&w[j]);
+          __nv_bfloat162 *ph = reinterpret_cast<__nv_bfloat162*>(&oh), *pm = reinterpret_cast<__nv_bfloat162*>(&om),
+                         *pl = reinterpret_cast<__nv_bfloat162*>(&ol);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float2 y;
-            unpack_bf16(in[i], y.x, y.y);
-            y = mul2(y, make_float2(f, f));
-            oh[i] = pack_bf16(y.x, y.y);
-            float2 t;
-            unpack_bf16(oh[i], t.x, t.y);
-            y = add2(y, make_float2(-t.x, -t.y));
-            om[i] = pack_bf16(y.x, y.y);
-            unpack_bf16(om[i], t.x, t.y);
-            y = add2(y, make_float2(-t.x, -t.y));
-            ol[i] = pack_bf16(y.x, y.y);
+            const __nv_bfloat162 hi = __hmul2_rn(in[i], f[0]), m = __hfma2(in[i], f[0], __hneg2(hi));
+            const __nv_bfloat162 mid = __hfma2(in[i], f[1], m);
+            ph[i] = hi;
+            pm[i] = mid;
+            pl[i] = __hfma2(in[i], f[2], __hfma2(in[i], f[1], __hsub2_rn(m, mid)));
           }
-          *reinterpret_cast<uint4*>(sVd + off) = make_uint4(oh[0], oh[1], oh[2], oh[3]);
-          *reinterpret_cast<uint4*>(sVd + BLK + off) = make_uint4(om[0], om[1], om[2], om[3]);
-          *reinterpret_cast<uint4*>(sVd + 2 * BLK + off) = make_uint4(ol[0], ol[1], ol[2], ol[3]);
+          uint8_t* dst = sVd + row + (((j0 + j) ^ sw) << 4);
+          *reinterpret_cast<uint4*>(dst) = oh;
+          *reinterpret_cast<uint4*>(dst + BLK) = om;
+          *reinterpret_cast<uint4*>(dst + 2 * BLK) = ol;
         }
       }
-      warp_arrive(&bars.vd_full, true);
-      if (local) {                                           // nothing else reads the v' tile: this role gives the stage back
-        named_bar_sync(3, 128);
-        if (q == 0 && lane == 0) mbar_arrive(&bars.v_empty[c & 1]);
-      }
+      warp_arrive(&bars.vd_full, true);                      // ends in a warp barrier: every lane has read its part of v'
+      if (lane == 0) mbar_arrive(local ? &bars.v_empty[c & 1] : &bars.v_read[c & 1]);
     }
-  } else if (!local) {
-    // ---- read-out: thread = row t ----
+  } else if (!local && warp < LT_W_LOAD) {
+    // ---- read-out: thread = row t; the tile leaves from the place of the v' tile ----
     const int t = q * 32 + lane;
+    const float fo = J.s_out * (steep ? 1.f : power(pw, rev ? LT_REV_C - t : t - LT_FWD_C));   // row factor
 #pragma unroll 1
     for (int c = 0; c < nch; ++c) {
       const int t0 = chunk_start(c), Tv = min(LT_T, s1 - t0);
-      uint8_t* out = sm + ((c & 1) * LT_STAGE + 4) * BLK;    // every reader of the v' tile is done once the accumulators are
-      const float fi = t < Tv ? J.s_in * pw[rev ? Tv - 1 - t : t + 1] : 0.f, fo = J.s_out;
-      const bool ok = role_wait(&bars.acc_full, (uint32_t)(c & 1), abort_flag, dead);
+      uint8_t* out = sm + ((c & 1) * LT_STAGE + 4) * BLK;
+      bool ok = role_wait(&bars.acc_full[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead);   // the product has read the v' tile ...
+      ok = role_wait(&bars.v_read[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead) && ok;    // ... and so has the scaling
       if (ok) {
         tc_fence_after_sync();
+        const uint32_t acc = tmem_addr(tbase, q * 32, LT_O + (steep ? 64 : (c & 1) * 64));
+        const float fi = steep && t < Tv ? J.s_in * pw[rev ? Tv - 1 - t : t + 1] : 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          uint32_t r[16], w[16];
-          tmem_ld16(tmem_addr(tbase, q * 32, LT_O + j * 16), r);
-          tmem_ld16(tmem_addr(tbase, q * 32, LT_O2 + j * 16), w);
+          uint32_t r[16], o[8];
+          tmem_ld16(acc + j * 16, r);
           tmem_ld_wait();
-          uint32_t o[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float2 v = fma2(make_float2(fi, fi), f2(w[2 * i], w[2 * i + 1]), mul2(make_float2(fo, fo), f2(r[2 * i], r[2 * i + 1])));
-            o[i] = pack_bf16(v.x, v.y);
+            const float2 v = mul2(make_float2(fo, fo), f2(r[2 * i], r[2 * i + 1]));
+            r[2 * i] = __float_as_uint(v.x);
+            r[2 * i + 1] = __float_as_uint(v.y);
           }
+          if (steep) {                                       // the carried part with a row factor of its own
+            uint32_t w[16];
+            tmem_ld16(tmem_addr(tbase, q * 32, LT_O + j * 16), w);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(fmaf(fi, __uint_as_float(w[i]), __uint_as_float(r[i])));
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = pack_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
           *reinterpret_cast<uint4*>(out + sw128_offset(t, 2 * j)) = make_uint4(o[0], o[1], o[2], o[3]);
           *reinterpret_cast<uint4*>(out + sw128_offset(t, 2 * j + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
         }
       }
-      warp_arrive(&bars.acc_empty, true);
+      warp_arrive(&bars.acc_empty[c & 1], true);
       named_bar_sync(2, 128);
-      if (tid == 12 * 32) {
+      if (tid == LT_W_OUT * 32) {
         if (ok) {
           tma_store_4d(my, out, e0, h, t0, b);
           bulk_commit_group();
@@ -404,12 +499,45 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         mbar_arrive(&bars.v_empty[c & 1]);
       }
     }
-    if (tid == 12 * 32) bulk_wait_group<0>();
+    if (tid == LT_W_OUT * 32) bulk_wait_group<0>();
   }
   tc_fence_before_sync();
   __syncthreads();
   if (tid == 0 && *abort_flag && p.status) atomicExch(p.status, 1);
   if (warp == 0) tmem_dealloc(tbase, 512);
+}
+
+__global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_constant__ LaTcArgs a, const int local) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ LtShared sh;
+  const LaPlan& p = a.p;
+  // tile index: e tile fastest, then job, segment, head, batch
+  int64_t id = blockIdx.x;
+  const int ne = p.ne;
+  const int et = (int)(id % ne);
+  id /= ne;
+  const int jb = (int)(id % p.njobs);
+  id /= p.njobs;
+  const int seg = (int)(id % p.nseg);
+  id /= p.nseg;
+  const int h = (int)(id % p.H), b = (int)(id / p.H);
+  const LaJob& J = p.job[jb];
+  const int rev = J.reverse;
+  if (et * LT_E >= J.E) return;
+  if (local && seg == (rev ? 0 : p.nseg - 1)) return;        // nobody reads the last segment's share
+  uint8_t* sm = align1024(smem_raw);
+  const double ld = (double)p.log_decay[h];
+  const bool steep = !(fabs(ld) <= 0.693147);
+  if (local) {
+    if (rev) la_tc_walk<true, false, true>(a, sh, sm, jb, b, h, seg, et, ld);
+    else la_tc_walk<false, false, true>(a, sh, sm, jb, b, h, seg, et, ld);
+  } else if (!steep) {
+    if (rev) la_tc_walk<true, false, false>(a, sh, sm, jb, b, h, seg, et, ld);
+    else la_tc_walk<false, false, false>(a, sh, sm, jb, b, h, seg, et, ld);
+  } else {
+    if (rev) la_tc_walk<true, true, false>(a, sh, sm, jb, b, h, seg, et, ld);
+    else la_tc_walk<false, true, false>(a, sh, sm, jb, b, h, seg, et, ld);
+  }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
