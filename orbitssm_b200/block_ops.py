@@ -5,7 +5,6 @@ C-ABI library on the current stream of the tensors' device.
 """
 from __future__ import annotations
 
-import contextlib
 from typing import NamedTuple
 
 import torch
@@ -15,7 +14,6 @@ from . import _lib, ops
 PACK_GROUP = 32      # elements of a row that share one exponent
 
 _DT = ops._DT
-_NULL = contextlib.nullcontext()
 
 
 def device_of(who, *tensors):
@@ -24,26 +22,53 @@ def device_of(who, *tensors):
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.device
+        if d.type != "cuda":
             ops._require_cuda(who, t)
+            raise ValueError(f"{who}: got a tensor on {d}; the kernels run on CUDA devices")
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{who}: tensors on {dev} and {t.device}; all of them have to be on one device")
+            dev = d
+        elif d != dev:
+            raise ValueError(f"{who}: tensors on {dev} and {d}; all of them have to be on one device")
     return dev
 
 
-def on(device):
-    """Context in which `device` is the current one (kernels launch there, whatever device the caller had current)."""
-    return _NULL if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def launch(name, launches, device, fn, *args):
+    """Call the C-ABI function `fn` with `args` and the current stream of `device`, with `device` current, counted as `launches`
+    kernels under `name`; a nonzero status raises."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return launch(name, launches, device, fn, *args)
+    if ops._TIMING is None:
+        ops.LAUNCHES += launches
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with ops._timed(name, launches):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if status:
+        _lib.check(status, fn.__name__)
 
 
-def raw_stream(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def wants_grad(*tensors):
+    """Is a gradient recorded for any of them?  Where none is, a call skips the autograd node (about 10 us of host time)."""
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
-def _count(launches):
-    ops.LAUNCHES += launches
+def same_device(who, dev, *tensors):
+    """Refuse (by name) unless every tensor is on CUDA device number `dev`."""
+    for t in tensors:
+        if t is not None and t.get_device() != dev or dev < 0:
+            device_of(who, *tensors)
+
+
+def like(t):
+    """A new dense tensor of the shape and type of `t`."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
 
 
 def io_code(who, t):
@@ -55,6 +80,13 @@ def io_code(who, t):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _weight(t):
+    """A weight vector as the kernels read it: dense float32."""
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return ops._f32(t)
 
 
 # ----------------------------------------------------------------------------------------------------
@@ -79,28 +111,26 @@ def _stride(t):
 def block_norm_fwd(x, h, gate, scale, w_post, w_pre, eps, keep):
     """x, h, gate [M, D] (gate may be None), weights fp32 [D] or None -> (r, n | None, rstd_h | None, rstd_r | None);
     the rstd are kept where `keep`."""
-    dev = device_of("block_norm", x, h, gate, scale, w_post, w_pre)
+    dev = x.device
     M, D = x.shape
-    r = torch.empty((M, D), device=dev, dtype=x.dtype)
-    n = torch.empty((M, D), device=dev, dtype=x.dtype) if w_pre is not None else None
+    r = like(x)
+    n = like(x) if w_pre is not None else None
     rh = torch.empty((M,), device=dev, dtype=torch.float32) if keep and w_post is not None else None
     rr = torch.empty((M,), device=dev, dtype=torch.float32) if keep and w_pre is not None else None
     if M:
-        with on(dev), ops._timed("block_norm_fwd", 1):
-            _lib.check(_lib.load().orbit_block_norm_fwd(
-                x.data_ptr(), _stride(x), h.data_ptr(), _stride(h), _ptr(gate), 0 if gate is None else _stride(gate),
-                _ptr(scale), _ptr(w_post), _ptr(w_pre), r.data_ptr(), _ptr(n), _ptr(rh), _ptr(rr), M, D, eps,
-                _DT[x.dtype], raw_stream(dev)), "orbit_block_norm_fwd")
+        launch("block_norm_fwd", 1, dev, _lib.load().orbit_block_norm_fwd, x.data_ptr(), _stride(x), h.data_ptr(), _stride(h),
+               _ptr(gate), 0 if gate is None else _stride(gate), _ptr(scale), _ptr(w_post), _ptr(w_pre), r.data_ptr(), _ptr(n),
+               _ptr(rh), _ptr(rr), M, D, eps, _DT[x.dtype])
     return r, n, rh, rr
 
 
 def block_norm_bwd(x, h, gate, scale, w_post, w_pre, rstd_h, rstd_r, dr, dn, want_sums=True):
     """Gradients of `block_norm_fwd`: (dx, dh, dgate | None, dscale | None, dw_post | None, dw_pre | None); dr or dn may
     be None (zeros).  Without `want_sums` the three column sums are left out."""
-    dev = device_of("block_norm", x, h, gate, scale, w_post, w_pre, dr, dn)
+    dev = device_of("block_norm", x, dr, dn)
     M, D = x.shape
     f32 = torch.float32
-    dx = torch.empty((M, D), device=dev, dtype=x.dtype)
+    dx = like(x)
     dh = torch.empty_like(dx)
     dg = torch.empty_like(dx) if gate is not None else None
     sums = [torch.empty((D,), device=dev, dtype=f32) if (want_sums and w is not None) else None for w in (scale, w_post, w_pre)]
@@ -109,13 +139,23 @@ def block_norm_bwd(x, h, gate, scale, w_post, w_pre, rstd_h, rstd_r, dr, dn, wan
     if any(s is not None for s in sums):
         nbytes = lib.orbit_block_norm_bwd_workspace_bytes(M, D)
         ws = torch.empty((nbytes,), device=dev, dtype=torch.uint8)
-    with on(dev), ops._timed("block_norm_bwd", (2 if ws is not None else 1) if M else 0):
-        _lib.check(lib.orbit_block_norm_bwd(
-            x.data_ptr(), _stride(x), h.data_ptr(), _stride(h), _ptr(gate), 0 if gate is None else _stride(gate), _ptr(scale),
-            _ptr(w_post), _ptr(w_pre), _ptr(rstd_h), _ptr(rstd_r), _ptr(dr), _ptr(dn), dx.data_ptr(), dh.data_ptr(), _ptr(dg),
-            _ptr(sums[0]), _ptr(sums[1]), _ptr(sums[2]), _ptr(ws), nbytes, M, D, _DT[x.dtype], raw_stream(dev)),
-            "orbit_block_norm_bwd")
+    launch("block_norm_bwd", (2 if ws is not None else 1) if M else 0, dev, lib.orbit_block_norm_bwd, x.data_ptr(), _stride(x),
+           h.data_ptr(), _stride(h), _ptr(gate), 0 if gate is None else _stride(gate), _ptr(scale), _ptr(w_post), _ptr(w_pre),
+           _ptr(rstd_h), _ptr(rstd_r), _ptr(dr), _ptr(dn), dx.data_ptr(), dh.data_ptr(), _ptr(dg), _ptr(sums[0]), _ptr(sums[1]),
+           _ptr(sums[2]), _ptr(ws), nbytes, M, D, _DT[x.dtype])
     return (dx, dh, dg, *sums)
+
+
+def _block_norm(x, h, gate, scale, w_post, w_pre, eps, keep):
+    """(r, n | None) in the shape of x, and what the backward pass reads."""
+    D = x.shape[-1]
+    x2, h2 = _rows_of(x, D), _rows_of(h, D)
+    g2 = None if gate is None else _rows_of(gate, D)
+    s32, wo, wi = _weight(scale), _weight(w_post), _weight(w_pre)
+    r, n, rh, rr = block_norm_fwd(x2, h2, g2, s32, wo, wi, eps, keep)
+    if x.dim() != 2:
+        r, n = r.view(x.shape), None if n is None else n.view(x.shape)
+    return r, n, (x2, h2, g2, s32, wo, wi, rh, rr)
 
 
 class BlockNormFn(torch.autograd.Function):
@@ -123,17 +163,11 @@ class BlockNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, h, gate, scale, w_post, w_pre, eps):
-        D = x.shape[-1]
-        x2, h2 = _rows_of(x, D), _rows_of(h, D)
-        g2 = None if gate is None else _rows_of(gate, D)
-        s32, wo, wi = ops._f32(scale), ops._f32(w_post), ops._f32(w_pre)
-        keep = any(ctx.needs_input_grad)
-        r, n, rh, rr = block_norm_fwd(x2, h2, g2, s32, wo, wi, eps, keep)
-        if keep:
-            ctx.set_materialize_grads(False)
-            ctx.save_for_backward(x2, h2, g2, s32, wo, wi, rh, rr)
-            ctx.meta = (x.shape, [None if t is None else t.dtype for t in (scale, w_post, w_pre)])
-        return r.view(x.shape), None if n is None else n.view(x.shape)
+        r, n, saved = _block_norm(x, h, gate, scale, w_post, w_pre, eps, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(*saved)
+        ctx.meta = (x.shape, [None if t is None else t.dtype for t in (scale, w_post, w_pre)])
+        return r, n
 
     @staticmethod
     @ops.first_order_only("block norm")
@@ -176,7 +210,9 @@ def block_norm(x, h, *, gate=None, scale=None, post_weight=None, pre_weight=None
             raise ValueError(f"{who}: {name} must be a floating [{x.shape[-1]}] vector, got {tuple(t.shape)}, {t.dtype}")
     if not eps >= 0:
         raise ValueError(f"{who}: eps must be at least 0, got {eps!r}")
-    device_of(who, x, h, gate, scale, post_weight, pre_weight)
+    same_device(who, x.get_device(), x, h, gate, scale, post_weight, pre_weight)
+    if not wants_grad(x, h, gate, scale, post_weight, pre_weight):
+        return _block_norm(x, h, gate, scale, post_weight, pre_weight, float(eps), False)[:2]
     return BlockNormFn.apply(x, h, gate, scale, post_weight, pre_weight, float(eps))
 
 
@@ -203,17 +239,16 @@ def pack_activation(x):
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"{who}: expected x [..., D] with D > 0, got {tuple(x.shape)}")
     code = io_code(who, x)
-    x = x.detach()
+    if x.requires_grad:
+        x = x.detach()
     dev = device_of(who, x)
     D = x.shape[-1]
     x2 = _rows_of(x, D)
     M = x2.shape[0]
-    q = torch.empty(x.shape, device=dev, dtype=torch.int8)
-    e = torch.empty((*x.shape[:-1], -(-D // PACK_GROUP)), device=dev, dtype=torch.uint8)
+    q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
+    e = q.new_empty((*x.shape[:-1], -(-D // PACK_GROUP)), dtype=torch.uint8)
     if M:
-        with on(dev), ops._timed("act_pack", 1):
-            _lib.check(_lib.load().orbit_act_pack(x2.data_ptr(), _stride(x2), q.data_ptr(), e.data_ptr(), M, D, code, raw_stream(dev)),
-                       "orbit_act_pack")
+        launch("act_pack", 1, dev, _lib.load().orbit_act_pack, x2.data_ptr(), _stride(x2), q.data_ptr(), e.data_ptr(), M, D, code)
     return PackedActivation(q, e, x.dtype)
 
 
@@ -230,12 +265,10 @@ def unpack_activation(packed, dtype=None):
                          f"{tuple(q.shape)} with {e.dtype} {tuple(e.shape)}")
     dev = device_of(who, q, e)
     q, e = q.contiguous(), e.contiguous()
-    x = torch.empty(q.shape, device=dev, dtype=dtype)
+    x = torch.empty_like(q, dtype=dtype)
     D = q.shape[-1]
     if q.numel():
-        with on(dev), ops._timed("act_unpack", 1):
-            _lib.check(_lib.load().orbit_act_unpack(q.data_ptr(), e.data_ptr(), x.data_ptr(), q.numel() // D, D, _DT[dtype],
-                                                    raw_stream(dev)), "orbit_act_unpack")
+        launch("act_unpack", 1, dev, _lib.load().orbit_act_unpack, q.data_ptr(), e.data_ptr(), x.data_ptr(), q.numel() // D, D, _DT[dtype])
     return x
 
 

@@ -11,13 +11,14 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from dataclasses import asdict, dataclass
 
 import torch
 import torch.nn as nn
 
 from . import _lib, ops
-from .block_ops import device_of, io_code, on, raw_stream
+from .block_ops import io_code, launch, like, same_device, wants_grad
 from .config import BACKENDS, PRECISIONS, _positive_int, _strict_from_dict, as_execution
 from .state import State, StateLifecycle
 
@@ -28,13 +29,17 @@ from .state import State, StateLifecycle
 def _operand(t):
     """`t` [B, L, H, D] as the kernels read it: a dense last axis; for bfloat16 heads of a multiple of 8 also 16-byte rows and no
     overlapping (expanded) axes, so that the tensor-core tiles can load it.  Copied only where it is not so already."""
+    D = t.shape[3]
+    tiles = t.dtype is torch.bfloat16 and D % 8 == 0
+    if t.is_contiguous():
+        return t if not tiles or t.data_ptr() % 16 == 0 else t.clone()
     sb, sl, sh, sd = t.stride()
-    if sd != 1 and t.shape[3] > 1:
+    if sd != 1 and D > 1:
         return t.contiguous()
-    if t.dtype == torch.bfloat16 and t.shape[3] % 8 == 0:
+    if tiles:
         if t.data_ptr() % 16:
             return t.clone(memory_format=torch.contiguous_format)
-        for n, s in ((t.shape[0], sb), (t.shape[1], sl), (t.shape[2], sh)):
+        for n, s in zip(t.shape, (sb, sl, sh)):
             if n > 1 and (s % 8 or s <= 0):
                 return t.contiguous()
     return t
@@ -42,85 +47,78 @@ def _operand(t):
 
 def _strides(t):
     """(batch, token, head) strides; an axis of one element, whose stride is never used, gets an aligned one."""
-    return tuple(s if n > 1 else 8 for n, s in zip(t.shape[:3], t.stride()[:3]))
+    B, L, H, D = t.shape
+    if t.is_contiguous():
+        return (L * H * D, H * D, D)
+    sb, sl, sh, _ = t.stride()
+    return (sb if B > 1 else 8, sl if L > 1 else 8, sh if H > 1 else 8)
 
 
 def _status(device):
-    if ("cuda", device.index) not in ops._STATUS and torch.cuda.is_current_stream_capturing():
-        return None                # the word must not be born in a graph's memory pool
+    if (device.type, device.index) not in ops._STATUS and torch.cuda.is_current_stream_capturing():
+        return 0                   # the word must not be born in a graph's memory pool
     return ops._status_word(device).data_ptr()
 
 
-def _args(q, k, v, log_decay, state, scale):
-    a = _lib.LaArgs()
-    a.B, a.L, a.H, a.Dk, a.Dv, a.scale = q.shape[0], q.shape[1], q.shape[2], q.shape[3], v.shape[3], scale
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_bs, a.q_ls, a.q_hs = _strides(q)
-    a.k_bs, a.k_ls, a.k_hs = _strides(k)
-    a.v_bs, a.v_ls, a.v_hs = _strides(v)
-    a.log_decay = log_decay.data_ptr()
-    if state is not None:
-        a.state0 = state.data_ptr()
-    a.status = _status(q.device)
-    return a
+#: `orbit_la_args` in one call: filling the ctypes structure field by field costs the host 6 us more
+_PACK = struct.Struct("@5if" + "P3q" * 3 + "PP" + "P3q" + "P" + "P3q" + "P" + "P3q" * 3 + "PPqP")
+assert _PACK.size == C.sizeof(_lib.LaArgs)
+_NONE = (0, 0, 0, 0)
 
 
-def _workspace(a, bwd, code, device):
-    nbytes = _lib.load().orbit_la_workspace_bytes(C.byref(a), bwd, code)
-    if not nbytes:
-        return None
-    ws = torch.empty((nbytes,), device=device, dtype=torch.uint8)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    return ws
+def _run(name, fn, bwd, q, k, v, log_decay, state, scale, code, tail):
+    """Pack the argument block (`tail`: its fields from `y` up to the workspace), ask for the workspace and launch."""
+    dev = q.device
+    B, L, H, Dk = q.shape
+    Dv = v.shape[3]
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _run(name, fn, bwd, q, k, v, log_decay, state, scale, code, tail)
+    fields = (B, L, H, Dk, Dv, scale, q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v),
+              log_decay.data_ptr(), 0 if state is None else state.data_ptr(), *tail)
+    status = _status(dev)
+    lib = _lib.load()
+    ws, nbytes = None, 0
+    if L > 32:                     # a sequence of one tile is never split, whatever the kernels
+        nbytes = lib.orbit_la_workspace_bytes(_PACK.pack(*fields, 0, 0, status), bwd, code)
+        if nbytes:
+            ws = torch.empty((nbytes,), device=dev, dtype=torch.uint8)
+    launch(name, 1 if ws is None else 2, dev, fn, _PACK.pack(*fields, 0 if ws is None else ws.data_ptr(), nbytes, status), code)
 
 
 def la_fwd(q, k, v, log_decay, state, scale, want_state):
     """Operands as `_operand` leaves them -> (y [B, L, H, Dv], state [B, H, Dv, Dk] | None)."""
-    dev = q.device
     B, L, H, Dk = q.shape
     Dv = v.shape[3]
-    y = torch.empty((B, L, H, Dv), device=dev, dtype=q.dtype)
-    new = torch.empty((B, H, Dv, Dk), device=dev, dtype=torch.float32) if want_state else None
-    if B == 0 or (L == 0 and not want_state):
-        return y, new
-    code = ops._DT[q.dtype]
-    with on(dev):
-        a = _args(q, k, v, log_decay, state, scale)
-        a.y = y.data_ptr()
-        a.y_bs, a.y_ls, a.y_hs = _strides(y)
-        if new is not None:
-            a.state1 = new.data_ptr()
-        ws = _workspace(a, 0, code, dev)  # noqa: F841 - alive until the launch is queued on this stream
-        with ops._timed("linear_attention_fwd", 1 if ws is None else 2):
-            _lib.check(_lib.load().orbit_la_fwd(C.byref(a), code, raw_stream(dev)), "orbit_la_fwd")
+    y = like(v)
+    new = None
+    if want_state:
+        new = torch.empty((B, H, Dv, Dk), device=q.device, dtype=torch.float32) if state is None else torch.empty_like(state)
+    if B and (L or want_state):
+        _run("linear_attention_fwd", _lib.load().orbit_la_fwd, 0, q, k, v, log_decay, state, scale, ops._DT[q.dtype],
+             (y.data_ptr(), L * H * Dv, H * Dv, Dv, 0 if new is None else new.data_ptr(), *_NONE, 0, *_NONE, *_NONE, *_NONE, 0))
     return y, new
 
 
 def la_bwd(q, k, v, log_decay, state, scale, dy, dstate, want_dstate0, outs=(None, None, None)):
     """Gradients (dq, dk, dv, dstate0 | None); `outs` may name tensors (any strides, dense last axis) that receive dq, dk, dv."""
-    dev = q.device
-    dq, dk, dv = (o if o is not None else torch.empty(t.shape, device=dev, dtype=t.dtype) for o, t in zip(outs, (q, k, v)))
+    dq, dk, dv = (like(t) if o is None else o for o, t in zip(outs, (q, k, v)))
     B, L, H, Dk = q.shape
-    ds0 = torch.empty((B, H, v.shape[3], Dk), device=dev, dtype=torch.float32) if want_dstate0 else None
-    if B == 0 or (L == 0 and not want_dstate0):
-        return dq, dk, dv, ds0
-    code = ops._DT[q.dtype]
-    with on(dev):
-        a = _args(q, k, v, log_decay, state, scale)
-        a.dy = dy.data_ptr()
-        a.dy_bs, a.dy_ls, a.dy_hs = _strides(dy)
-        if dstate is not None:
-            a.dstate1 = dstate.data_ptr()
-        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        a.dq_bs, a.dq_ls, a.dq_hs = _strides(dq)
-        a.dk_bs, a.dk_ls, a.dk_hs = _strides(dk)
-        a.dv_bs, a.dv_ls, a.dv_hs = _strides(dv)
-        if ds0 is not None:
-            a.dstate0 = ds0.data_ptr()
-        ws = _workspace(a, 1, code, dev)  # noqa: F841
-        with ops._timed("linear_attention_bwd", 1 if ws is None else 2):
-            _lib.check(_lib.load().orbit_la_bwd(C.byref(a), code, raw_stream(dev)), "orbit_la_bwd")
+    ds0 = torch.empty((B, H, v.shape[3], Dk), device=q.device, dtype=torch.float32) if want_dstate0 else None
+    if B and (L or want_dstate0):
+        _run("linear_attention_bwd", _lib.load().orbit_la_bwd, 1, q, k, v, log_decay, state, scale, ops._DT[q.dtype],
+             (*_NONE, 0, dy.data_ptr(), *_strides(dy), 0 if dstate is None else dstate.data_ptr(), dq.data_ptr(), *_strides(dq),
+              dk.data_ptr(), *_strides(dk), dv.data_ptr(), *_strides(dv), 0 if ds0 is None else ds0.data_ptr()))
     return dq, dk, dv, ds0
+
+
+def _la(q, k, v, log_decay, state, scale, want_state):
+    """(y, state | None) and what the backward pass reads."""
+    q, k, v = _operand(q), _operand(k), _operand(v)
+    if state is not None and not state.is_contiguous():
+        state = state.contiguous()
+    y, new = la_fwd(q, k, v, log_decay, state, scale, want_state)
+    return y, new, (q, k, v, log_decay, state)
 
 
 class LinearAttentionFn(torch.autograd.Function):
@@ -128,13 +126,10 @@ class LinearAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, scale, want_state, slots):
-        q, k, v = _operand(q), _operand(k), _operand(v)
-        s0 = None if state is None else state.detach().contiguous()
-        y, new = la_fwd(q, k, v, log_decay, s0, scale, want_state)
-        if any(ctx.needs_input_grad):
-            ctx.set_materialize_grads(False)
-            ctx.save_for_backward(q, k, v, log_decay, s0)
-            ctx.scale, ctx.slots = scale, slots
+        y, new, saved = _la(q, k, v, log_decay, state, scale, want_state)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(*saved)
+        ctx.scale, ctx.slots = scale, slots
         return y, new
 
     @staticmethod
@@ -161,24 +156,24 @@ class LinearAttentionFn(torch.autograd.Function):
 
 def _check_operands(who, q, k, v, log_decay, state, lead):
     """Shapes, dtypes and device of a call; `lead` names the axes before the heads."""
-    n = len(lead)
-    if q.dim() != n + 2 or k.shape != q.shape or v.dim() != n + 2 or v.shape[:-1] != q.shape[:-1]:
+    qs, vs = q.shape, v.shape
+    if len(qs) != len(lead) + 2 or k.shape != qs or len(vs) != len(qs) or vs[:-1] != qs[:-1]:
         axes = ", ".join(lead)
         raise ValueError(f"{who}: expected q, k [{axes}, H, Dk] and v [{axes}, H, Dv] (as many key heads as query heads: expand shared "
-                         f"heads), got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+                         f"heads), got {tuple(qs)}, {tuple(k.shape)}, {tuple(vs)}")
     code = io_code(who, q)
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"{who}: q, k and v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
-    H, Dk, Dv = q.shape[-2], q.shape[-1], v.shape[-1]
+    B, H, Dk, Dv = qs[0], qs[-2], qs[-1], vs[-1]
     if H < 1 or not 1 <= Dk <= 256 or not 1 <= Dv <= 256:
         raise NotImplementedError(f"{who}: at least one head, of widths 1..256, got H={H} Dk={Dk} Dv={Dv}")
-    if log_decay.dim() != 1 or log_decay.shape[0] != H or log_decay.dtype != torch.float32:
+    if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
         raise ValueError(f"{who}: log_decay must be float32 [{H}], got {log_decay.dtype} {tuple(log_decay.shape)}")
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{who}: log_decay is a constant of the layer; its gradient is not served (detach it)")
-    if state is not None and (tuple(state.shape) != (q.shape[0], H, Dv, Dk) or state.dtype != torch.float32):
-        raise ValueError(f"{who}: state must be float32 {(q.shape[0], H, Dv, Dk)}, got {state.dtype} {tuple(state.shape)}")
-    device_of(who, q, k, v, log_decay, state)
+    if state is not None and (state.shape != (B, H, Dv, Dk) or state.dtype != torch.float32):
+        raise ValueError(f"{who}: state must be float32 {(B, H, Dv, Dk)}, got {state.dtype} {tuple(state.shape)}")
+    same_device(who, q.get_device(), q, k, v, log_decay, state)
     return code
 
 
@@ -204,8 +199,13 @@ def linear_attention(q, k, v, log_decay, state=None, *, scale=None, return_state
     float32 kernels.  Values are expected to be finite: a NaN or infinity may reach every output of its head and sequence."""
     who = "linear_attention"
     _check_operands(who, q, k, v, log_decay, state, ("B", "L"))
-    y, new = LinearAttentionFn.apply(q, k, v, log_decay.detach().contiguous(), state, _scale_of(who, scale, q.shape[-1]),
-                                     bool(return_state), _slots)
+    scale, return_state = _scale_of(who, scale, q.shape[-1]), bool(return_state)
+    if not log_decay.is_contiguous() or log_decay.requires_grad:
+        log_decay = log_decay.detach().contiguous()
+    if wants_grad(q, k, v, state):
+        y, new = LinearAttentionFn.apply(q, k, v, log_decay, state, scale, return_state, _slots)
+    else:
+        y, new, _ = _la(q, k, v, log_decay, state, scale, return_state)
     return (y, new) if return_state else y
 
 
@@ -218,7 +218,7 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out_state=No
     if state is None:
         raise ValueError(f"{who}: a state is required (zeros before the first token)")
     code = _check_operands(who, q, k, v, log_decay, state, ("B",))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+    if wants_grad(q, k, v, state):
         raise ValueError(f"{who}: gradients are not served; use linear_attention on a sequence of one token, or torch.no_grad()")
     if out_state is not None and (out_state.shape != state.shape or out_state.dtype != torch.float32 or not out_state.is_contiguous()
                                   or out_state.device != state.device):
@@ -226,19 +226,25 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out_state=No
     scale = _scale_of(who, scale, q.shape[-1])
     B, H, Dk = q.shape
     Dv, dev = v.shape[2], q.device
-    q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
-    state = state.contiguous()
+    q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
+    if not state.is_contiguous():
+        state = state.contiguous()
     if out_state is not None and out_state.data_ptr() != state.data_ptr() and _overlap(out_state, state):
         raise ValueError(f"{who}: out_state overlaps state without being it")
     new = torch.empty_like(state) if out_state is None else out_state
-    y = torch.empty((B, H, Dv), device=dev, dtype=q.dtype)
+    y = like(v)
     if B:
-        with on(dev), ops._timed("linear_attention_step", 1):
-            _lib.check(_lib.load().orbit_la_step(
-                q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                v.stride(1), log_decay.contiguous().data_ptr(), state.data_ptr(), new.data_ptr(), y.data_ptr(), B, H, Dk, Dv, scale, code,
-                raw_stream(dev)), "orbit_la_step")
+        qb, qh, _ = q.stride()
+        kb, kh, _ = k.stride()
+        vb, vh, _ = v.stride()
+        launch("linear_attention_step", 1, dev, _lib.load().orbit_la_step, q.data_ptr(), qb, qh, k.data_ptr(), kb, kh, v.data_ptr(), vb,
+               vh, (log_decay if log_decay.is_contiguous() else log_decay.contiguous()).data_ptr(), state.data_ptr(), new.data_ptr(),
+               y.data_ptr(), B, H, Dk, Dv, scale, code)
     return y, new
+
+
+def _dense_rows(t):
+    return t if t.shape[2] == 1 or t.stride(2) == 1 else t.contiguous()
 
 
 def _overlap(a, b):
