@@ -20,12 +20,15 @@
 // (no atomics: reproducible).
 //
 // HBM-bound: forward (2 + gate) reads and 2 writes of es bytes an element, backward (4 + gate) reads and (2 + gate) writes.
+// Measured at [65536, 2048] bfloat16 with every factor: forward 227 us (5.9 TB/s, 90 % of the copy bandwidth), backward 419 us
+// (5.1 TB/s, 78 %: one barrier a row at two CTAs of 256 threads an SM, registers allow no third).
 #include "common.cuh"
 #include "../../include/orbit_b200.h"
 
 namespace orbit {
 
-constexpr int BN_THREADS = 256;
+constexpr int BN_THREADS = 256;                              // of the scalar kernels
+__host__ __device__ constexpr int bn_threads(int tpr) { return tpr > 256 ? tpr : 256; }   // a CTA: one wide row, or several narrow ones
 
 struct BnArgs {
   const void *x, *h, *g;
@@ -48,7 +51,7 @@ __device__ __forceinline__ float bn_sigmoid(float x) { return __fdividef(1.f, 1.
 // Sums of K values over the TPR threads of a row, by TPR consecutive threads; every thread of the row gets them.  `red`
 // holds K values for each warp of the CTA; callers alternate two buffers so that one barrier a call is enough.
 template <int TPR, int K>
-__device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[BN_THREADS / 32]) {
+__device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[bn_threads(TPR) / 32]) {
 #pragma unroll
   for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
   if constexpr (TPR > 32) {
@@ -70,69 +73,104 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[BN_THREADS /
 }
 
 
-// Forward.  TPR threads a row, NV 16-byte vectors a thread and tensor, 256 / TPR rows a CTA, all loads before the first use.
-template <typename T, int TPR, int NV, bool GATE>
-__global__ void __launch_bounds__(BN_THREADS) block_norm_fwd_kernel(const BnArgs a) {
-  constexpr int V = Vec16<T>::N, ROWS = BN_THREADS / TPR;
-  __shared__ float red[2][1][BN_THREADS / 32];
-  const int lt = threadIdx.x % TPR, D = a.D;
-  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
-  const bool live = row < a.M;
-  Vec16<T> rx[NV], rh[NV], rg[GATE ? NV : 1];
+// The weights of this thread's columns, kept in registers over the rows of a CTA: js = scale w_post and w_pre.  (Read for every
+// row they were the kernel's bound: eight floats a lane, 32 bytes apart, are eight wavefronts a load.)
+template <int V, int TPR, int NV>
+__device__ __forceinline__ void load_weights(const BnArgs& a, int lt, float (&js)[NV][V], float (&wp)[NV][V]) {
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (k * TPR + lt) * V;
-    if (live && c < D) {
-      rh[k].load((const T*)a.h + row * a.hrs + c);
-      rx[k].load((const T*)a.x + row * a.xrs + c);
-      if (GATE) rg[GATE ? k : 0].load((const T*)a.g + row * a.grs + c);
+    if (c < a.D) {
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
+        const float4 u = a.scale ? *reinterpret_cast<const float4*>(a.scale + c + i) : one;
+        const float4 w = a.wpost ? *reinterpret_cast<const float4*>(a.wpost + c + i) : one;
+        const float4 p = a.wpre ? *reinterpret_cast<const float4*>(a.wpre + c + i) : one;
+        js[k][i] = u.x * w.x; js[k][i + 1] = u.y * w.y; js[k][i + 2] = u.z * w.z; js[k][i + 3] = u.w * w.w;
+        wp[k][i] = p.x; wp[k][i + 1] = p.y; wp[k][i + 2] = p.z; wp[k][i + 3] = p.w;
+      }
     }
   }
+}
+
+// Forward.  TPR threads a row, NV 16-byte vectors a thread and tensor, 256 / TPR rows at a time; a CTA walks row groups
+// blockIdx.x, blockIdx.x + gridDim.x, ..., the loads of the next one in flight over the sums and stores of the current one.
+template <typename T, int TPR, int NV, bool GATE>
+__global__ void __launch_bounds__(bn_threads(TPR), NV > 1 || TPR > 256 ? 1 : 3) block_norm_fwd_kernel(const BnArgs a) {
+  constexpr int V = Vec16<T>::N, ROWS = bn_threads(TPR) / TPR;
+  __shared__ float red[4][1][bn_threads(TPR) / 32];               // two sums a row group, two groups
+  const int lt = threadIdx.x % TPR, sub = threadIdx.x / TPR, D = a.D;
+  const int64_t stride = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + sub;
+  Vec16<T> nx[NV], nh[NV], ng[GATE ? NV : 1];
+  auto fetch = [&](int64_t r) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + lt) * V;
+      if (r < a.M && c < D) {
+        nh[k].load((const T*)a.h + r * a.hrs + c);
+        if (GATE) ng[GATE ? k : 0].load((const T*)a.g + r * a.grs + c);
+        nx[k].load((const T*)a.x + r * a.xrs + c);
+      }
+    }
+  };
+  fetch(row);
+  float js[NV][V], wp[NV][V];
+  load_weights<V, TPR, NV>(a, lt, js, wp);
   const float invD = 1.f / (float)D;
-  float rs_h = 1.f;
-  if (a.wpost) {
-    float ss[1] = {0.f};
+  int par = 0;
+#pragma unroll 1
+  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.M; row0 += stride, row += stride, par ^= 2) {
+    const bool live = row < a.M;
+    float m[NV][V], r[NV][V], ss[1] = {0.f}, s2[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if (live && (k * TPR + lt) * V < D) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) ss[0] = fmaf(rh[k].get(i), rh[k].get(i), ss[0]);
+        for (int i = 0; i < V; ++i) {
+          const float hv = nh[k].get(i);
+          ss[0] = fmaf(hv, hv, ss[0]);
+          m[k][i] = hv * js[k][i];
+          if (GATE) m[k][i] *= bn_sigmoid(ng[GATE ? k : 0].get(i));
+          r[k][i] = nx[k].get(i);
+        }
       }
     }
-    row_sum<TPR, 1>(ss, red[0]);
-    rs_h = rsqrtf(fmaf(ss[0], invD, a.eps));
-    if (live && lt == 0 && a.rstd_h) a.rstd_h[row] = rs_h;
-  }
-  float r[NV][V], s2[1] = {0.f};
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (k * TPR + lt) * V;
-    if (live && c < D) {
-      Vec16<T> o;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float m = rh[k].get(i);
-        if (a.wpost) m = m * rs_h * a.wpost[c + i];
-        if (GATE) m *= bn_sigmoid(rg[GATE ? k : 0].get(i));
-        r[k][i] = fmaf(a.scale ? a.scale[c + i] : 1.f, m, rx[k].get(i));
-        s2[0] = fmaf(r[k][i], r[k][i], s2[0]);
-        o.set(i, r[k][i]);
-      }
-      o.store((T*)a.r + row * (int64_t)D + c);
+    fetch(row + stride);
+    float rs_h = 1.f;
+    if (a.wpost) {
+      row_sum<TPR, 1>(ss, red[par]);
+      rs_h = rsqrtf(fmaf(ss[0], invD, a.eps));
+      if (live && lt == 0 && a.rstd_h) a.rstd_h[row] = rs_h;
     }
-  }
-  if (!a.wpre) return;
-  row_sum<TPR, 1>(s2, red[1]);
-  const float rs_r = rsqrtf(fmaf(s2[0], invD, a.eps));
-  if (live && lt == 0 && a.rstd_r) a.rstd_r[row] = rs_r;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (k * TPR + lt) * V;
-    if (live && c < D) {
-      Vec16<T> o;
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + lt) * V;
+      if (live && c < D) {
+        Vec16<T> o;
 #pragma unroll
-      for (int i = 0; i < V; ++i) o.set(i, r[k][i] * rs_r * a.wpre[c + i]);
-      o.store((T*)a.n + row * (int64_t)D + c);
+        for (int i = 0; i < V; ++i) {
+          r[k][i] = fmaf(rs_h, m[k][i], r[k][i]);
+          s2[0] = fmaf(r[k][i], r[k][i], s2[0]);
+          o.set(i, r[k][i]);
+        }
+        o.store((T*)a.r + row * (int64_t)D + c);
+      }
+    }
+    if (!a.wpre) continue;
+    row_sum<TPR, 1>(s2, red[par + 1]);
+    const float rs_r = rsqrtf(fmaf(s2[0], invD, a.eps));
+    if (live && lt == 0 && a.rstd_r) a.rstd_r[row] = rs_r;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + lt) * V;
+      if (live && c < D) {
+        Vec16<T> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.set(i, r[k][i] * rs_r * wp[k][i]);
+        o.store((T*)a.n + row * (int64_t)D + c);
+      }
     }
   }
 }
@@ -140,9 +178,10 @@ __global__ void __launch_bounds__(BN_THREADS) block_norm_fwd_kernel(const BnArgs
 // Backward.  A CTA walks row groups blockIdx.x, blockIdx.x + gridDim.x, ...; the next group's loads are issued before the
 // barrier of the current one.
 template <typename T, int TPR, int NV, bool GATE>
-__global__ void __launch_bounds__(BN_THREADS) block_norm_bwd_kernel(const BnArgs a) {
-  constexpr int V = Vec16<T>::N, ROWS = BN_THREADS / TPR;
-  __shared__ float red[2][3][BN_THREADS / 32];
+__global__ void __launch_bounds__(bn_threads(TPR), NV > 1 || TPR > 256 ? 1 : 2) block_norm_bwd_kernel(const BnArgs a) {
+  constexpr int V = Vec16<T>::N, ROWS = bn_threads(TPR) / TPR;
+  __shared__ float red[2][3][bn_threads(TPR) / 32];
+  __shared__ float cols[ROWS > 1 ? 2 * ROWS * TPR * V : 1];  // column sums of the CTA's row groups (narrow rows)
   const int lt = threadIdx.x % TPR, D = a.D;
   const float invD = 1.f / (float)D;
   float acc_a[NV][V], acc_p[NV][V];
@@ -168,6 +207,8 @@ __global__ void __launch_bounds__(BN_THREADS) block_norm_bwd_kernel(const BnArgs
   const int sub = threadIdx.x / TPR;
   int par = 0;
   if (first < a.M) fetch(first + sub);
+  float js[NV][V], wp[NV][V];
+  load_weights<V, TPR, NV>(a, lt, js, wp);
   for (int64_t row0 = first; row0 < a.M; row0 += stride, par ^= 1) {
     const int64_t row = row0 + sub;
     const bool live = row < a.M;
@@ -182,7 +223,7 @@ __global__ void __launch_bounds__(BN_THREADS) block_norm_bwd_kernel(const BnArgs
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           hh[k][i] = rh[k].get(i) * rs_h;
-          float j = hh[k][i] * (a.scale ? a.scale[c + i] : 1.f) * (a.wpost ? a.wpost[c + i] : 1.f);
+          float j = hh[k][i] * js[k][i];
           if (GATE) {
             sg[GATE ? k : 0][i] = bn_sigmoid(rg[GATE ? k : 0].get(i));
             j *= sg[GATE ? k : 0][i];
@@ -191,7 +232,7 @@ __global__ void __launch_bounds__(BN_THREADS) block_norm_bwd_kernel(const BnArgs
           q[k][i] = 0.f;
           if (a.dn) {
             q[k][i] = (rx[k].get(i) + j) * rs_r;
-            const float dn = rdn[k].get(i), w = dn * a.wpre[c + i];
+            const float dn = rdn[k].get(i), w = dn * wp[k][i];
             acc_p[k][i] = fmaf(dn, q[k][i], acc_p[k][i]);
             sum[0] = fmaf(w, q[k][i], sum[0]);
             sum[2] = fmaf(q[k][i], j, sum[2]);
@@ -211,13 +252,12 @@ __global__ void __launch_bounds__(BN_THREADS) block_norm_bwd_kernel(const BnArgs
         Vec16<T> ox, oh, og;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float s = a.scale ? a.scale[c + i] : 1.f, wp = a.wpost ? a.wpost[c + i] : 1.f;
           const float d = fmaf(-c1, q[k][i], e[k][i]);
           const float sig = GATE ? sg[GATE ? k : 0][i] : 1.f;
           const float t = d * sig;                               // gradient of r through the gate
           acc_a[k][i] = fmaf(t, hh[k][i], acc_a[k][i]);
           ox.set(i, d);
-          const float dm = t * s * wp;
+          const float dm = t * js[k][i];
           if (GATE) og.set(i, dm * hh[k][i] * (1.f - sig));
           oh.set(i, a.wpost ? rs_h * (dm - hh[k][i] * c2) : dm);
         }
@@ -227,16 +267,33 @@ __global__ void __launch_bounds__(BN_THREADS) block_norm_bwd_kernel(const BnArgs
       }
     }
   }
-  // partial column sums [slot][2][D], a slot for each row group of the CTA
-  const int64_t slot = (int64_t)blockIdx.x * ROWS + sub;
+  // partial column sums [slot][2][D], a slot for each CTA; its row groups are added in order
+  if (a.part == nullptr) return;
+  float* part = a.part + (int64_t)blockIdx.x * 2 * D;
+  if constexpr (ROWS > 1) {
+    static_assert(NV == 1, "several rows a CTA hold one vector a thread");
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (k * TPR + lt) * V;
-    if (a.part && c < D) {
+    for (int i = 0; i < V; ++i) {
+      cols[(sub * 2) * TPR * V + lt * V + i] = acc_a[0][i];
+      cols[(sub * 2 + 1) * TPR * V + lt * V + i] = acc_p[0][i];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * D; c += bn_threads(TPR)) {
+      const int which = c >= D, col = c - which * D;
+      float t = 0.f;
+      for (int r = 0; r < ROWS; ++r) t += cols[(r * 2 + which) * TPR * V + col];
+      part[c] = t;
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        a.part[(slot * 2) * D + c + i] = acc_a[k][i];
-        a.part[(slot * 2 + 1) * D + c + i] = acc_p[k][i];
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + lt) * V;
+      if (c < D) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          part[c + i] = acc_a[k][i];
+          part[D + c + i] = acc_p[k][i];
+        }
       }
     }
   }
@@ -361,14 +418,14 @@ __global__ void __launch_bounds__(256) block_norm_colsum_kernel(const float* __r
 }
 
 // 16-byte vectors a row takes -> threads a row and vectors a thread (0: the scalar kernels).  A row keeps to one warp up to 32
-// vectors and spreads over a whole CTA beyond 128, so that a thread holds few registers and many rows are in flight.
+// vectors and spreads over up to 512 threads, so that a thread holds few registers and many rows are in flight.
 struct BnShape { int tpr, nv; };
 static BnShape bn_shape(int vectors) {
   if (vectors <= 32) return {32, 1};
   if (vectors <= 64) return {64, 1};
   if (vectors <= 128) return {128, 1};
   if (vectors <= 256) return {256, 1};
-  if (vectors <= 512) return {256, 2};
+  if (vectors <= 512) return {512, 1};
   if (vectors <= 1024) return {256, 4};
   return {0, 0};
 }
@@ -377,34 +434,35 @@ template <typename T>
 static bool bn_vectors(const BnArgs& a, bool bwd, BnShape* s) {
   constexpr int V = Vec16<T>::N;
   bool ok = a.D % V == 0 && a.xrs % V == 0 && a.hrs % V == 0 && (!a.g || a.grs % V == 0) && aligned16(a.x) && aligned16(a.h) &&
-            aligned16(a.g);
+            aligned16(a.g) && aligned16(a.scale) && aligned16(a.wpost) && aligned16(a.wpre);
   if (bwd) ok = ok && aligned16(a.dr) && aligned16(a.dn) && aligned16(a.dx) && aligned16(a.dh) && aligned16(a.dg);
   else ok = ok && aligned16(a.r) && aligned16(a.n);
   *s = bn_shape((a.D + V - 1) / V);
   return ok && s->tpr > 0;
 }
 
-// Row groups that walk in the backward pass: four CTAs' worth an SM; every slot is written in full before it is read.
-static int64_t bn_slots(int64_t M) { return M < 592 ? (M > 0 ? M : 1) : 592; }
+// CTAs that walk in the backward pass: two to an SM; every slot is written in full before it is read.
+constexpr int BN_SLOTS = 148 * 2;
+static int64_t bn_slots(int64_t M) { return M < BN_SLOTS ? (M > 0 ? M : 1) : BN_SLOTS; }
 
 #define BN_DISPATCH(KERNEL, GRID)                                                              \
   do {                                                                                         \
     const int key = s.tpr * 8 + s.nv;                                                          \
     const unsigned grid = (unsigned)(GRID);                                                    \
     if (a.g) {                                                                                 \
-      if (key == 32 * 8 + 1) KERNEL<T, 32, 1, true><<<grid, BN_THREADS, 0, st>>>(a);           \
-      else if (key == 64 * 8 + 1) KERNEL<T, 64, 1, true><<<grid, BN_THREADS, 0, st>>>(a);      \
-      else if (key == 128 * 8 + 1) KERNEL<T, 128, 1, true><<<grid, BN_THREADS, 0, st>>>(a);    \
-      else if (key == 256 * 8 + 1) KERNEL<T, 256, 1, true><<<grid, BN_THREADS, 0, st>>>(a);    \
-      else if (key == 256 * 8 + 2) KERNEL<T, 256, 2, true><<<grid, BN_THREADS, 0, st>>>(a);    \
-      else KERNEL<T, 256, 4, true><<<grid, BN_THREADS, 0, st>>>(a);                            \
+      if (key == 32 * 8 + 1) KERNEL<T, 32, 1, true><<<grid, bn_threads(32), 0, st>>>(a);           \
+      else if (key == 64 * 8 + 1) KERNEL<T, 64, 1, true><<<grid, bn_threads(64), 0, st>>>(a);      \
+      else if (key == 128 * 8 + 1) KERNEL<T, 128, 1, true><<<grid, bn_threads(128), 0, st>>>(a);    \
+      else if (key == 256 * 8 + 1) KERNEL<T, 256, 1, true><<<grid, bn_threads(256), 0, st>>>(a);    \
+      else if (key == 512 * 8 + 1) KERNEL<T, 512, 1, true><<<grid, bn_threads(512), 0, st>>>(a);    \
+      else KERNEL<T, 256, 4, true><<<grid, bn_threads(256), 0, st>>>(a);                            \
     } else {                                                                                   \
-      if (key == 32 * 8 + 1) KERNEL<T, 32, 1, false><<<grid, BN_THREADS, 0, st>>>(a);          \
-      else if (key == 64 * 8 + 1) KERNEL<T, 64, 1, false><<<grid, BN_THREADS, 0, st>>>(a);     \
-      else if (key == 128 * 8 + 1) KERNEL<T, 128, 1, false><<<grid, BN_THREADS, 0, st>>>(a);   \
-      else if (key == 256 * 8 + 1) KERNEL<T, 256, 1, false><<<grid, BN_THREADS, 0, st>>>(a);   \
-      else if (key == 256 * 8 + 2) KERNEL<T, 256, 2, false><<<grid, BN_THREADS, 0, st>>>(a);   \
-      else KERNEL<T, 256, 4, false><<<grid, BN_THREADS, 0, st>>>(a);                           \
+      if (key == 32 * 8 + 1) KERNEL<T, 32, 1, false><<<grid, bn_threads(32), 0, st>>>(a);          \
+      else if (key == 64 * 8 + 1) KERNEL<T, 64, 1, false><<<grid, bn_threads(64), 0, st>>>(a);     \
+      else if (key == 128 * 8 + 1) KERNEL<T, 128, 1, false><<<grid, bn_threads(128), 0, st>>>(a);   \
+      else if (key == 256 * 8 + 1) KERNEL<T, 256, 1, false><<<grid, bn_threads(256), 0, st>>>(a);   \
+      else if (key == 512 * 8 + 1) KERNEL<T, 512, 1, false><<<grid, bn_threads(512), 0, st>>>(a);   \
+      else KERNEL<T, 256, 4, false><<<grid, bn_threads(256), 0, st>>>(a);                           \
     }                                                                                          \
   } while (0)
 
@@ -412,9 +470,9 @@ template <typename T>
 static int block_norm_fwd_t(const BnArgs& a, cudaStream_t st) {
   BnShape s;
   if (bn_vectors<T>(a, false, &s)) {
-    const int rows = BN_THREADS / s.tpr;
-    const int64_t blocks = (a.M + rows - 1) / rows;
-    ORBIT_REQUIRE(blocks <= 0x7fffffffLL, ERR_UNSUPPORTED, "orbit_block_norm_fwd: %lld rows are too many for one call", (long long)a.M);
+    const int rows = bn_threads(s.tpr) / s.tpr;
+    const int64_t groups = (a.M + rows - 1) / rows, most = s.nv > 1 || s.tpr > 256 ? 148 : 148 * 3;   // what the SMs hold at once
+    const int64_t blocks = groups < most ? groups : most;
     BN_DISPATCH(block_norm_fwd_kernel, blocks);
     ORBIT_CHECK_LAUNCH("block_norm_fwd_kernel");
     return OK;
@@ -429,10 +487,9 @@ static int block_norm_bwd_t(const BnArgs& a, float* dscale, float* dwpost, float
   BnShape s;
   int64_t slots;
   if (bn_vectors<T>(a, true, &s)) {
-    const int rows = BN_THREADS / s.tpr;
-    const int64_t blocks = bn_slots((a.M + rows - 1) / rows);
-    slots = blocks * rows;
-    BN_DISPATCH(block_norm_bwd_kernel, blocks);
+    const int rows = bn_threads(s.tpr) / s.tpr;
+    slots = bn_slots((a.M + rows - 1) / rows);
+    BN_DISPATCH(block_norm_bwd_kernel, slots);
     ORBIT_CHECK_LAUNCH("block_norm_bwd_kernel");
   } else {
     slots = bn_slots(a.M);
@@ -467,9 +524,7 @@ extern "C" int orbit_block_norm_fwd(const void* x, int64_t x_row_stride, const v
 }
 
 extern "C" int64_t orbit_block_norm_bwd_workspace_bytes(int64_t M, int D) {
-  // at most 592 CTAs of at most 8 row groups, two partial sums a column each
-  const int64_t rows = M < 592 * 8 ? (M > 0 ? M + 8 : 8) : 592 * 8;
-  return rows * 2 * D * (int64_t)sizeof(float);
+  return bn_slots(M) * 2 * D * (int64_t)sizeof(float);
 }
 
 extern "C" int orbit_block_norm_bwd(const void* x, int64_t x_row_stride, const void* h, int64_t h_row_stride, const void* gate,
