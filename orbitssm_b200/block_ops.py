@@ -280,21 +280,17 @@ class CheckpointFn(torch.autograd.Function):
     def forward(ctx, block, x, *params):
         ctx.block = block
         ctx.amp = (torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda"))
-        ctx.versions = [p._version for p in params]
         packed = pack_activation(x)
         ctx.dtype = x.dtype
         with torch.no_grad():
             y = block(x)
-        ctx.save_for_backward(packed.q, packed.exponent, *params)
+        ctx.save_for_backward(packed.q, packed.exponent, *params)     # the parameters: a change in place before the backward is refused
         return y
 
     @staticmethod
     @ops.first_order_only("8-bit activation checkpoint")
     def backward(ctx, dy):
         q, e, *params = ctx.saved_tensors
-        if [p._version for p in params] != ctx.versions:
-            raise RuntimeError("8-bit activation checkpoint: a parameter of the block was changed in place between the forward "
-                               "and the backward pass; the block cannot be run again as it was")
         x = unpack_activation(PackedActivation(q, e, ctx.dtype)).requires_grad_(ctx.needs_input_grad[1])
         wanted = [p for p, need in zip(params, ctx.needs_input_grad[2:]) if need]
         ins = ([x] if ctx.needs_input_grad[1] else []) + wanted

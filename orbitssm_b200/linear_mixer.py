@@ -334,6 +334,14 @@ class LinearAttention(StateLifecycle, nn.Module):
         self._final_state = None
         self.set_execution(as_execution(execution))
 
+    def _apply(self, fn, recurse=True):
+        """Moves and casts the layer; the decays stay float32 (``.to(torch.bfloat16)`` would move a span of 4096 tokens by 8)."""
+        kept = self.log_decay
+        super()._apply(fn, recurse)
+        if self.log_decay.dtype != torch.float32:
+            self.log_decay = kept.to(self.log_decay.device)
+        return self
+
     # -- execution ------------------------------------------------------------------------------------------
     def _check_execution(self, ex):
         f, out = ex.fields(), {}

@@ -130,6 +130,11 @@ def test_layer_configuration():
     for ex in ({"precision": "ieee"}, {"chunk_size": 64}, {"checkpoint": True}, {"kernel_options": {"a": 1}}, {"backend": "torch"}):
         with pytest.raises(ValueError):
             ob.LinearAttention(c, ex)
+    kept = layer.log_decay.clone()
+    layer.to(BF)
+    assert layer.q_proj.weight.dtype == BF and layer.log_decay.dtype == F32 and torch.equal(layer.log_decay, kept)
+    layer.load_state_dict(ob.LinearAttention(c).state_dict())
+    layer.float()
     with pytest.raises(ValueError, match="CPU tensor"):
         layer(torch.zeros(1, 3, 64))
     with pytest.raises(ValueError, match="expected x"):
