@@ -173,6 +173,26 @@ def load():
     return lib
 
 
+_host = None
+_HOST_ENTRIES = ("orbit_la_step", "orbit_la_fwd", "orbit_la_workspace_bytes", "orbit_block_norm_fwd", "orbit_act_pack", "orbit_act_unpack",
+                 "orbit_la_bwd")
+
+
+def host():
+    """The native host calls of the block operators (``csrc/host_calls.cpp``), bound to this library's entry points."""
+    global _host
+    if _host is None:
+        lib = load()
+        try:
+            from . import _orbit_host
+        except ImportError as e:
+            raise OrbitLibraryError(f"the extension module _orbit_host cannot be loaded ({e}): build it with "
+                                    "`python -m orbitssm_b200.build`") from e
+        _orbit_host.bind(*[C.cast(getattr(lib, n), C.c_void_p).value for n in _HOST_ENTRIES])
+        _host = _orbit_host
+    return _host
+
+
 def check(status: int, who: str):
     """Raise the Python exception that matches a nonzero status (the message is the library's own text)."""
     if status == 0:

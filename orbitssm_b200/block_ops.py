@@ -49,6 +49,20 @@ def launch(name, launches, device, fn, *args):
         _lib.check(status, fn.__name__)
 
 
+def native(name, *args):
+    """The outputs of host call `name` (`_lib.host`), or None where it leaves the call to the Python way."""
+    if ops._TIMING is not None:
+        return None                    # a timed region needs the events around the launch
+    got = getattr(_lib._host or _lib.host(), name)(*args)
+    if got is None:
+        return None
+    *outs, status, launches = got
+    if status:
+        _lib.check(status, name)
+    ops.LAUNCHES += launches
+    return outs
+
+
 def wants_grad(*tensors):
     """Is a gradient recorded for any of them?  Where none is, a call skips the autograd node (about 10 us of host time)."""
     if not torch.is_grad_enabled():
@@ -197,6 +211,9 @@ def block_norm(x, h, *, gate=None, scale=None, post_weight=None, pre_weight=None
     x, h, gate: [..., D] of one shape and dtype (float32 or bfloat16; a column slice of a wider buffer is read in place);
     scale, post_weight, pre_weight: [D].  Returns (r, n) in the dtype of x; arithmetic, norms and the weights' gradients are
     float32, and n is formed from the unrounded r.  First-order differentiable in every tensor argument."""
+    got = native("block_norm", x, h, gate, scale, post_weight, pre_weight, eps)
+    if got is not None:
+        return tuple(got)
     who = "block_norm"
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"{who}: expected x [..., D] with D > 0, got {tuple(x.shape)}")
@@ -235,6 +252,9 @@ def pack_activation(x):
     two for each 32 elements of a row, the least under which the group's largest element rounds to at most 127 (never below
     2^-126).  Rounding is to nearest, ties to even: off by at most half a step, and a step is at most 1/64 of the group's
     largest element (values within 2^122 of the type's largest are off by up to a step, so as to stay finite).  A non-finite element is restored as NaN and leaves its group's scale alone.  Not differentiable."""
+    got = native("pack", x)
+    if got is not None:
+        return PackedActivation(*got, x.dtype)
     who = "pack_activation"
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"{who}: expected x [..., D] with D > 0, got {tuple(x.shape)}")
@@ -259,6 +279,9 @@ def unpack_activation(packed, dtype=None):
     dtype = own_dtype if dtype is None else dtype
     if dtype not in _DT:
         raise NotImplementedError(f"{who}: activations must be float32 or bfloat16, got {dtype}")
+    got = native("unpack", q, e, dtype is torch.bfloat16)
+    if got is not None:
+        return got[0]
     if q.dtype != torch.int8 or e.dtype != torch.uint8 or q.dim() < 1 or q.shape[-1] == 0 \
             or tuple(e.shape) != (*q.shape[:-1], -(-q.shape[-1] // PACK_GROUP)):
         raise ValueError(f"{who}: expected int8 q [..., D] with uint8 exponents [..., ceil(D / {PACK_GROUP})], got {q.dtype} "

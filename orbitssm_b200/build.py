@@ -1,11 +1,13 @@
 """Build ``liborbit_b200.so`` in-tree with nvcc for sm_100a:  ``python -m orbitssm_b200.build``.
 
 Each ``csrc/*.cu`` is compiled to an object file under ``csrc/_obj`` (in parallel, and only when it or a header is newer
-than its object), then the objects are linked into the shared library next to this file."""
+than its object), then the objects are linked into the shared library next to this file.  ``csrc/host_calls.cpp`` (host code
+against the headers of the installed torch, no kernels) becomes the extension module ``_orbit_host.so`` beside it."""
 from __future__ import annotations
 
 import glob
 import os
+import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -14,6 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "_obj")
 OUT = os.path.join(HERE, "liborbit_b200.so")
+HOST_SRC, HOST_OUT = os.path.join(CSRC, "host_calls.cpp"), os.path.join(HERE, "_orbit_host.so")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 
 
@@ -41,7 +44,29 @@ def stale() -> bool:
     return _newer(OUT, sources() + headers())
 
 
+def build_host(force: bool = False) -> str:
+    """The host-call extension (C++ against torch's headers; the torch libraries are found when the module is loaded)."""
+    if not force and not _newer(HOST_OUT, [HOST_SRC, os.path.join(os.path.dirname(HERE), "include", "orbit_b200.h")]):
+        return HOST_OUT
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    nvcc = os.environ.get("NVCC", "nvcc")
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(shutil.which(nvcc) or "/usr/local/cuda/bin/nvcc")))
+    inc = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *["-I" + i for i in inc], HOST_SRC, "-o", HOST_OUT, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch",
+           "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+    return HOST_OUT
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    build_host(force)
     if not force and not stale():
         return OUT
     nvcc = os.environ.get("NVCC", "nvcc")

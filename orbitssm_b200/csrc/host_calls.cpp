@@ -1,0 +1,328 @@
+// Host side of the block operators' calls that record no gradient: checks, output tensors and the launch in one native call.
+//
+// A call of these operators on small inputs (one token, one decode batch) costs the host several times what it costs the GPU;
+// checks and ctypes in Python are most of it (measured on the B200 host, us a call: step 16, block norm 17, pack 12, unpack 9).
+// Each function here serves the ordinary call and returns None for every other one (a CPU tensor, mixed dtypes, a gradient to
+// record, operands that would have to be copied, ...); the Python operator then takes its own way, which serves the call or refuses
+// it by name.  The kernels and the C-ABI entry points are the same on both ways; this file holds no arithmetic.
+#include <Python.h>
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+
+#include "../../include/orbit_b200.h"
+
+namespace {
+
+// entry points of liborbit_b200.so, handed over as addresses (the library is loaded once, by ctypes)
+struct Entry {
+  decltype(&orbit_la_step) la_step;
+  decltype(&orbit_la_fwd) la_fwd;
+  decltype(&orbit_la_bwd) la_bwd;
+  decltype(&orbit_la_workspace_bytes) la_workspace;
+  decltype(&orbit_block_norm_fwd) block_norm;
+  decltype(&orbit_act_pack) pack;
+  decltype(&orbit_act_unpack) unpack;
+} entry = {};
+
+// a plain torch.Tensor (no subclass) on the current CUDA device for which no gradient is to be recorded
+bool plain(PyObject* o, at::Tensor& t, int device) {
+  if (!THPVariable_CheckExact(o)) return false;
+  t = THPVariable_Unpack(o);
+  return t.is_cuda() && t.get_device() == device && !(t.requires_grad() && c10::GradMode::is_enabled()) && t.layout() == at::kStrided;
+}
+bool plain_or_none(PyObject* o, at::Tensor& t, int device) { return o == Py_None || plain(o, t, device); }
+
+int io_code(const at::Tensor& t) {
+  return t.scalar_type() == at::kBFloat16 ? ORBIT_BF16 : t.scalar_type() == at::kFloat ? ORBIT_F32 : -1;
+}
+// the current device, or -1 for a call whose first operand does not live on a CUDA device (there may be none at all)
+int device_for(PyObject* first) {
+  if (c10::impl::dispatch_mode_enabled() || !THPVariable_CheckExact(first) || !THPVariable_Unpack(first).is_cuda()) return -1;
+  return c10::cuda::current_device();
+}
+void* stream(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
+template <typename T> T* ptr(const at::Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
+bool f32_vector(const at::Tensor& t, int64_t n) {
+  return !t.defined() || (t.dim() == 1 && t.size(0) == n && t.scalar_type() == at::kFloat && t.is_contiguous());
+}
+
+// the word of each device that a kernel sets when a bounded wait gives up (owned by the Python side)
+constexpr int MAX_DEVICES = 64;
+int* status_word[MAX_DEVICES] = {};
+
+// (outputs..., status, launches): the caller raises for a nonzero status
+PyObject* result(int status, const at::Tensor& a, const at::Tensor& b, int launches = 1) {
+  PyObject* x = THPVariable_Wrap(a);
+  PyObject* y = b.defined() ? THPVariable_Wrap(b) : Py_NewRef(Py_None);
+  PyObject* s = PyLong_FromLong(status);
+  PyObject* l = PyLong_FromLong(launches);
+  PyObject* out = (x && y && s && l) ? PyTuple_Pack(4, x, y, s, l) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  Py_XDECREF(s);
+  Py_XDECREF(l);
+  return out;
+}
+
+#define GUARDED(...)                                         \
+  try {                                                      \
+    __VA_ARGS__                                              \
+  } catch (const std::exception& e) {                        \
+    PyErr_SetString(PyExc_RuntimeError, e.what());           \
+    return nullptr;                                          \
+  }
+
+// the state and the decays of a call: [B, H, Dv, Dk] and [H] float32, dense
+bool state_ok(const at::Tensor& s, int64_t B, int64_t H, int64_t Dv, int64_t Dk) {
+  return s.dim() == 4 && s.size(0) == B && s.size(1) == H && s.size(2) == Dv && s.size(3) == Dk && s.scalar_type() == at::kFloat && s.is_contiguous();
+}
+
+// the scale of a call: None is 1 / sqrt(Dk); false where the other way has to refuse it
+bool scale_of(PyObject* o, int64_t Dk, double& scale) {
+  if (o == Py_None) {
+    scale = 1. / std::sqrt((double)Dk);
+    return true;
+  }
+  scale = PyFloat_AsDouble(o);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return std::isfinite(scale) && scale != 0.;
+}
+
+// step(q, k, v, log_decay, state, scale | None)
+PyObject* la_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) Py_RETURN_NONE;
+  GUARDED({
+    const int dev = device_for(a[0]);
+    if (dev < 0) Py_RETURN_NONE;
+    at::Tensor q, k, v, ld, s;
+    if (!plain(a[0], q, dev) || !plain(a[1], k, dev) || !plain(a[2], v, dev) || !plain(a[3], ld, dev) || !plain(a[4], s, dev)) Py_RETURN_NONE;
+    const int code = io_code(q);
+    if (code < 0 || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() || q.dim() != 3 || v.dim() != 3 ||
+        k.sizes() != q.sizes() || v.size(0) != q.size(0) || v.size(1) != q.size(1))
+      Py_RETURN_NONE;
+    const int64_t B = q.size(0), H = q.size(1), Dk = q.size(2), Dv = v.size(2);
+    double scale;
+    if (B < 1 || H < 1 || Dk < 1 || Dv < 1 || Dk > 256 || Dv > 256 || !f32_vector(ld, H) || !state_ok(s, B, H, Dv, Dk) || !v.is_contiguous() ||
+        q.stride(2) != 1 || k.stride(2) != 1 || B * H > (1 << 24) || !scale_of(a[5], Dk, scale))
+      Py_RETURN_NONE;
+    at::Tensor y = at::empty_like(v), s1 = at::empty_like(s);
+    const int rc = entry.la_step(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                 v.stride(1), ptr<float>(ld), ptr<float>(s), ptr<float>(s1), y.data_ptr(), (int)B, (int)H, (int)Dk, (int)Dv,
+                                 (float)scale, code, stream(dev));
+    return result(rc, y, s1);
+  })
+}
+
+// attention(q, k, v, log_decay, state | None, scale | None, return_state) of dense operands
+PyObject* la_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 7) Py_RETURN_NONE;
+  GUARDED({
+    const int dev = device_for(a[0]);
+    if (dev < 0) Py_RETURN_NONE;
+    if (dev >= MAX_DEVICES || status_word[dev] == nullptr) Py_RETURN_NONE;
+    at::Tensor q, k, v, ld, s;
+    if (!plain(a[0], q, dev) || !plain(a[1], k, dev) || !plain(a[2], v, dev) || !plain(a[3], ld, dev) || !plain_or_none(a[4], s, dev)) Py_RETURN_NONE;
+    const int code = io_code(q);
+    if (code < 0 || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() || q.dim() != 4 || v.dim() != 4 ||
+        k.sizes() != q.sizes() || v.size(0) != q.size(0) || v.size(1) != q.size(1) || v.size(2) != q.size(2))
+      Py_RETURN_NONE;
+    const int64_t B = q.size(0), L = q.size(1), H = q.size(2), Dk = q.size(3), Dv = v.size(3);
+    double scale;
+    const bool want = PyObject_IsTrue(a[6]) == 1;
+    if (B < 1 || L < 1 || L > (1 << 30) || H < 1 || Dk < 1 || Dv < 1 || Dk > 256 || Dv > 256 || B * H > (1 << 24) || !f32_vector(ld, H) ||
+        (s.defined() && !state_ok(s, B, H, Dv, Dk)) || !q.is_contiguous() || !k.is_contiguous() || !v.is_contiguous() ||
+        !scale_of(a[5], Dk, scale))
+      Py_RETURN_NONE;
+    auto address = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
+    if (code == ORBIT_BF16 && (address(q) % 16 || address(k) % 16 || address(v) % 16)) Py_RETURN_NONE;   // copied on the other way
+    at::Tensor y = at::empty_like(v), s1;
+    if (want) s1 = s.defined() ? at::empty_like(s) : at::empty({B, H, Dv, Dk}, q.options().dtype(at::kFloat));
+    orbit_la_args p = {};
+    p.B = (int)B; p.L = (int)L; p.H = (int)H; p.Dk = (int)Dk; p.Dv = (int)Dv; p.scale = (float)scale;
+    p.q = q.data_ptr(); p.q_bs = L * H * Dk; p.q_ls = H * Dk; p.q_hs = Dk;
+    p.k = k.data_ptr(); p.k_bs = L * H * Dk; p.k_ls = H * Dk; p.k_hs = Dk;
+    p.v = v.data_ptr(); p.v_bs = L * H * Dv; p.v_ls = H * Dv; p.v_hs = Dv;
+    p.y = y.data_ptr(); p.y_bs = L * H * Dv; p.y_ls = H * Dv; p.y_hs = Dv;
+    p.log_decay = ptr<float>(ld);
+    p.state0 = ptr<float>(s);
+    p.state1 = ptr<float>(s1);
+    p.status = status_word[dev];
+    at::Tensor ws;
+    p.workspace_bytes = entry.la_workspace(&p, 0, code);
+    if (p.workspace_bytes) {
+      ws = at::empty({p.workspace_bytes}, q.options().dtype(at::kByte));
+      p.workspace = ws.data_ptr();
+    }
+    const int rc = entry.la_fwd(&p, code, stream(dev));
+    return result(rc, y, s1, p.workspace_bytes ? 2 : 1);
+  })
+}
+
+// attention_bwd(q, k, v, log_decay, state | None, scale, dy, dstate | None, want dstate0) -> (dq, dk, dv, dstate0 | None, status, launches)
+PyObject* la_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 9) Py_RETURN_NONE;
+  GUARDED({
+    const int dev = device_for(a[0]);
+    if (dev < 0 || dev >= MAX_DEVICES || status_word[dev] == nullptr) Py_RETURN_NONE;
+    at::Tensor q, k, v, ld, s, dy, ds;
+    if (!plain(a[0], q, dev) || !plain(a[1], k, dev) || !plain(a[2], v, dev) || !plain(a[3], ld, dev) || !plain_or_none(a[4], s, dev) ||
+        !plain(a[6], dy, dev) || !plain_or_none(a[7], ds, dev))
+      Py_RETURN_NONE;
+    const int code = io_code(q);
+    double scale;
+    const bool want = PyObject_IsTrue(a[8]) == 1;
+    // q, k, v, log_decay and state are what the forward pass checked and kept
+    const int64_t B = q.size(0), L = q.size(1), H = q.size(2), Dk = q.size(3), Dv = v.size(3);
+    if (code < 0 || B < 1 || L < 1 || !scale_of(a[5], Dk, scale) || !q.is_contiguous() || !k.is_contiguous() || !v.is_contiguous() ||
+        dy.sizes() != v.sizes() || dy.scalar_type() != v.scalar_type() || !dy.is_contiguous() || (ds.defined() && !state_ok(ds, B, H, Dv, Dk)))
+      Py_RETURN_NONE;
+    auto address = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
+    if (code == ORBIT_BF16 && (address(q) % 16 || address(k) % 16 || address(v) % 16 || address(dy) % 16)) Py_RETURN_NONE;
+    at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v), ds0;
+    if (want) ds0 = at::empty({B, H, Dv, Dk}, q.options().dtype(at::kFloat));
+    orbit_la_args p = {};
+    p.B = (int)B; p.L = (int)L; p.H = (int)H; p.Dk = (int)Dk; p.Dv = (int)Dv; p.scale = (float)scale;
+    p.q = q.data_ptr(); p.dq = dq.data_ptr(); p.k = k.data_ptr(); p.dk = dk.data_ptr();
+    p.v = v.data_ptr(); p.dv = dv.data_ptr(); p.dy = dy.data_ptr();
+    p.q_bs = p.dq_bs = p.k_bs = p.dk_bs = L * H * Dk;
+    p.q_ls = p.dq_ls = p.k_ls = p.dk_ls = H * Dk;
+    p.q_hs = p.dq_hs = p.k_hs = p.dk_hs = Dk;
+    p.v_bs = p.dv_bs = p.dy_bs = L * H * Dv;
+    p.v_ls = p.dv_ls = p.dy_ls = H * Dv;
+    p.v_hs = p.dv_hs = p.dy_hs = Dv;
+    p.log_decay = ptr<float>(ld);
+    p.state0 = ptr<float>(s);
+    p.dstate1 = ptr<float>(ds);
+    p.dstate0 = ptr<float>(ds0);
+    p.status = status_word[dev];
+    at::Tensor ws;
+    p.workspace_bytes = entry.la_workspace(&p, 1, code);
+    if (p.workspace_bytes) {
+      ws = at::empty({p.workspace_bytes}, q.options().dtype(at::kByte));
+      p.workspace = ws.data_ptr();
+    }
+    const int rc = entry.la_bwd(&p, code, stream(dev));
+    PyObject* o[6] = {THPVariable_Wrap(dq), THPVariable_Wrap(dk), THPVariable_Wrap(dv), ds0.defined() ? THPVariable_Wrap(ds0) : Py_NewRef(Py_None),
+                      PyLong_FromLong(rc), PyLong_FromLong(p.workspace_bytes ? 2 : 1)};
+    PyObject* out = o[0] && o[1] && o[2] && o[3] && o[4] && o[5] ? PyTuple_Pack(6, o[0], o[1], o[2], o[3], o[4], o[5]) : nullptr;
+    for (PyObject* x : o) Py_XDECREF(x);
+    return out;
+  })
+}
+
+// block_norm(x, h, gate | None, scale | None, post | None, pre | None, eps) of dense operands
+PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 7) Py_RETURN_NONE;
+  GUARDED({
+    const int dev = device_for(a[0]);
+    if (dev < 0) Py_RETURN_NONE;
+    at::Tensor x, h, g, sc, post, pre;
+    if (!plain(a[0], x, dev) || !plain(a[1], h, dev) || !plain_or_none(a[2], g, dev) || !plain_or_none(a[3], sc, dev) ||
+        !plain_or_none(a[4], post, dev) || !plain_or_none(a[5], pre, dev))
+      Py_RETURN_NONE;
+    const int code = io_code(x);
+    const double eps = PyFloat_AsDouble(a[6]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    if (code < 0 || x.dim() < 1 || x.numel() == 0 || x.size(-1) > (1 << 30) || !x.is_contiguous() || h.sizes() != x.sizes() || h.scalar_type() != x.scalar_type() ||
+        !h.is_contiguous() || (g.defined() && (g.sizes() != x.sizes() || g.scalar_type() != x.scalar_type() || !g.is_contiguous())) || !(eps >= 0.))
+      Py_RETURN_NONE;
+    const int64_t D = x.size(-1), M = x.numel() / D;
+    if (!f32_vector(sc, D) || !f32_vector(post, D) || !f32_vector(pre, D)) Py_RETURN_NONE;
+    at::Tensor r = at::empty_like(x), y;
+    if (pre.defined()) y = at::empty_like(x);
+    const int rc = entry.block_norm(x.data_ptr(), D, h.data_ptr(), D, ptr<void>(g), D, ptr<float>(sc), ptr<float>(post), ptr<float>(pre),
+                                    r.data_ptr(), ptr<void>(y), nullptr, nullptr, M, (int)D, (float)eps, code, stream(dev));
+    return result(rc, r, y);
+  })
+}
+
+// pack(x) of a dense activation -> (q, exponent, status)
+PyObject* pack(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 1) Py_RETURN_NONE;
+  GUARDED({
+    const int dev = device_for(a[0]);
+    if (dev < 0) Py_RETURN_NONE;
+    at::Tensor x = THPVariable_Unpack(a[0]);
+    if (x.get_device() != dev || x.layout() != at::kStrided) Py_RETURN_NONE;
+    const int code = io_code(x);
+    if (code < 0 || x.dim() < 1 || x.numel() == 0 || x.size(-1) > (1 << 30) || !x.is_contiguous()) Py_RETURN_NONE;
+    const int64_t D = x.size(-1), M = x.numel() / D;
+    auto shape = x.sizes().vec();
+    at::Tensor q = at::empty(shape, x.options().dtype(at::kChar));
+    shape.back() = (D + 31) / 32;
+    at::Tensor e = at::empty(shape, x.options().dtype(at::kByte));
+    const int rc = entry.pack(x.data_ptr(), D, q.data_ptr(), e.data_ptr(), M, (int)D, code, stream(dev));
+    return result(rc, q, e);
+  })
+}
+
+// unpack(q, exponent, bfloat16?) of dense tensors -> (x, None, status)
+PyObject* unpack(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 3) Py_RETURN_NONE;
+  GUARDED({
+    const int dev = device_for(a[0]);
+    if (dev < 0) Py_RETURN_NONE;
+    at::Tensor q, e;
+    if (!plain(a[0], q, dev) || !plain(a[1], e, dev)) Py_RETURN_NONE;
+    if (q.scalar_type() != at::kChar || e.scalar_type() != at::kByte || q.dim() < 1 || q.numel() == 0 || q.size(-1) > (1 << 30) || !q.is_contiguous() ||
+        !e.is_contiguous() || e.dim() != q.dim() || e.size(-1) != (q.size(-1) + 31) / 32 ||
+        e.sizes().slice(0, e.dim() - 1) != q.sizes().slice(0, q.dim() - 1))
+      Py_RETURN_NONE;
+    const bool half = PyObject_IsTrue(a[2]) == 1;
+    const int64_t D = q.size(-1);
+    at::Tensor x = at::empty(q.sizes(), q.options().dtype(half ? at::kBFloat16 : at::kFloat));
+    const int rc = entry.unpack(q.data_ptr(), e.data_ptr(), x.data_ptr(), q.numel() / D, (int)D, half ? ORBIT_BF16 : ORBIT_F32, stream(dev));
+    return result(rc, x, at::Tensor());
+  })
+}
+
+// bind(addresses of the entry points, in the order of `Entry`)
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  void* p[7];
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "bind takes seven addresses");
+    return nullptr;
+  }
+  for (int i = 0; i < 7; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
+  if (PyErr_Occurred()) return nullptr;
+  entry.la_step = reinterpret_cast<decltype(entry.la_step)>(p[0]);
+  entry.la_fwd = reinterpret_cast<decltype(entry.la_fwd)>(p[1]);
+  entry.la_workspace = reinterpret_cast<decltype(entry.la_workspace)>(p[2]);
+  entry.block_norm = reinterpret_cast<decltype(entry.block_norm)>(p[3]);
+  entry.pack = reinterpret_cast<decltype(entry.pack)>(p[4]);
+  entry.unpack = reinterpret_cast<decltype(entry.unpack)>(p[5]);
+  entry.la_bwd = reinterpret_cast<decltype(entry.la_bwd)>(p[6]);
+  Py_RETURN_NONE;
+}
+
+// bind_status(device, address of its status word)
+PyObject* bind_status(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 2) {
+    PyErr_SetString(PyExc_TypeError, "bind_status takes a device number and an address");
+    return nullptr;
+  }
+  const long dev = PyLong_AsLong(a[0]);
+  void* p = PyLong_AsVoidPtr(a[1]);
+  if (PyErr_Occurred()) return nullptr;
+  if (dev >= 0 && dev < MAX_DEVICES) status_word[dev] = static_cast<int*>(p);
+  Py_RETURN_NONE;
+}
+
+#define METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {METHOD("bind", bind),     METHOD("la_step", la_step), METHOD("la_fwd", la_fwd), METHOD("block_norm", block_norm),
+                         METHOD("pack", pack),     METHOD("unpack", unpack),
+                         METHOD("bind_status", bind_status), METHOD("la_bwd", la_bwd), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_orbit_host", "Native host calls of the block operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__orbit_host(void) { return PyModule_Create(&module); }

@@ -18,7 +18,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, ops
-from .block_ops import io_code, launch, like, same_device, wants_grad
+from .block_ops import io_code, launch, like, native, same_device, wants_grad
 from .config import BACKENDS, PRECISIONS, _positive_int, _strict_from_dict, as_execution
 from .state import State, StateLifecycle
 
@@ -57,7 +57,9 @@ def _strides(t):
 def _status(device):
     if (device.type, device.index) not in ops._STATUS and torch.cuda.is_current_stream_capturing():
         return 0                   # the word must not be born in a graph's memory pool
-    return ops._status_word(device).data_ptr()
+    word = ops._status_word(device).data_ptr()
+    _lib.host().bind_status(device.index, word)
+    return word
 
 
 #: `orbit_la_args` in one call: filling the ctypes structure field by field costs the host 6 us more
@@ -88,6 +90,9 @@ def _run(name, fn, bwd, q, k, v, log_decay, state, scale, code, tail):
 
 def la_fwd(q, k, v, log_decay, state, scale, want_state):
     """Operands as `_operand` leaves them -> (y [B, L, H, Dv], state [B, H, Dv, Dk] | None)."""
+    got = native("la_fwd", q, k, v, log_decay, state, scale, want_state)
+    if got is not None:
+        return got
     B, L, H, Dk = q.shape
     Dv = v.shape[3]
     y = like(v)
@@ -102,6 +107,10 @@ def la_fwd(q, k, v, log_decay, state, scale, want_state):
 
 def la_bwd(q, k, v, log_decay, state, scale, dy, dstate, want_dstate0, outs=(None, None, None)):
     """Gradients (dq, dk, dv, dstate0 | None); `outs` may name tensors (any strides, dense last axis) that receive dq, dk, dv."""
+    if outs[0] is None and outs[1] is None and outs[2] is None:
+        got = native("la_bwd", q, k, v, log_decay, state, scale, dy, dstate, want_dstate0)
+        if got is not None:
+            return got
     dq, dk, dv = (like(t) if o is None else o for o, t in zip(outs, (q, k, v)))
     B, L, H, Dk = q.shape
     ds0 = torch.empty((B, H, v.shape[3], Dk), device=q.device, dtype=torch.float32) if want_dstate0 else None
@@ -197,6 +206,9 @@ def linear_attention(q, k, v, log_decay, state=None, *, scale=None, return_state
     bfloat16 heads whose widths are multiples of 8 up to 128 run on tensor-core tiles: products of the unrounded inputs with the
     scores or the state rounded once to bfloat16, float32 sums; the state itself is float32 throughout.  Other calls run on
     float32 kernels.  Values are expected to be finite: a NaN or infinity may reach every output of its head and sequence."""
+    got = native("la_fwd", q, k, v, log_decay, state, scale, return_state)
+    if got is not None:
+        return tuple(got) if return_state else got[0]
     who = "linear_attention"
     _check_operands(who, q, k, v, log_decay, state, ("B", "L"))
     scale, return_state = _scale_of(who, scale, q.shape[-1]), bool(return_state)
@@ -214,6 +226,10 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out_state=No
 
     `out_state` (contiguous float32 of the state's shape) receives the new state; it may be `state` itself.  For inference: not
     differentiable (run `linear_attention` on a sequence of one token for gradients).  Everything else as there."""
+    if out_state is None:
+        got = native("la_step", q, k, v, log_decay, state, scale)
+        if got is not None:
+            return tuple(got)
     who = "linear_attention_step"
     if state is None:
         raise ValueError(f"{who}: a state is required (zeros before the first token)")

@@ -439,3 +439,63 @@ def test_pack_reads_strided_rows():
         got = ob.unpack_activation(ob.pack_activation(view))
         assert got.shape == view.shape and torch.equal(got, ob.unpack_activation(ob.pack_activation(view.contiguous())))
     assert ob.unpack_activation(ob.pack_activation(x[:0])).shape == (0, 300)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+#  the two ways to a launch
+# ---------------------------------------------------------------------------------------------------------------------
+def test_native_host_calls_and_the_python_way_give_the_same_bits():
+    g = _gen(40)
+    for dtype in (BF, F32):
+        q, k, v, ld, s0, dy, ds1 = _inputs(2, 300, 2, 64, 72, dtype, 41)
+        x, w = _randn(g, 5, 7, 96, dtype=dtype), _randn(g, 96)
+
+        def run():
+            leaves = [t.clone().requires_grad_(True) for t in (q, k, v, s0)]
+            y, s = ob.linear_attention(*leaves[:3], ld, leaves[3], return_state=True)
+            out = [y, s, *torch.autograd.grad((y, s), leaves, (dy, ds1))]
+            with torch.no_grad():
+                out += ob.linear_attention(q, k, v, ld, s0, scale=0.3, return_state=True)
+                out += ob.linear_attention_step(q[:, 0].contiguous(), k[:, 0].contiguous(), v[:, 0].contiguous(), ld, s0)
+                out += ob.block_norm(x, x, gate=x, scale=w, post_weight=w, pre_weight=w)
+                out.append(ob.block_norm(x, x)[0])
+                p = ob.pack_activation(x)
+                out += [p.q, p.exponent, ob.unpack_activation(p), ob.unpack_activation(p, F32)]
+            return out
+
+        native = run()
+        launches = ops.LAUNCHES
+        run()
+        launches = ops.LAUNCHES - launches
+        timed = []
+        ops.set_timing(timed)                             # a timed region takes the Python way
+        try:
+            before = ops.LAUNCHES
+            python = run()
+            assert ops.LAUNCHES - before == launches and timed
+        finally:
+            ops.set_timing(None)
+        assert len(native) == len(python) and all(torch.equal(a, b) for a, b in zip(native, python))
+
+
+def test_calls_on_tensors_of_another_type_or_place_are_refused_on_the_gpu_too():
+    q, k, v, ld, s0, _, _ = _inputs(1, 4, 2, 8, 8, F32, 42)
+    with pytest.raises(ValueError, match="one dtype"):
+        ob.linear_attention(q, k.to(BF), v, ld)
+    with pytest.raises(ValueError, match="CPU tensor|one device"):
+        ob.linear_attention(q, k.cpu(), v, ld)
+    with pytest.raises(ValueError, match="CPU tensor|one device"):
+        ob.block_norm(q, q, pre_weight=torch.ones(8))
+    with pytest.raises(ValueError, match="scale must be finite"):
+        ob.linear_attention(q, k, v, ld, scale=float("inf"))
+    with pytest.raises(ValueError, match="gradients are not served"):
+        ob.linear_attention_step(q[:, 0].clone().requires_grad_(True), k[:, 0], v[:, 0], ld, s0)
+    with pytest.raises(ValueError, match="out_state"):
+        ob.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s0, out_state=s0[:, :1])
+    both = torch.zeros(3, 2, 8, 8, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        ob.linear_attention_step(*(t[:, 0].expand(2, 2, 8) for t in (q, k, v)), ld, both[:2], out_state=both[1:])
+    with pytest.raises(RuntimeError, match="second-order"):
+        qq = q.clone().requires_grad_(True)
+        g, = torch.autograd.grad(ob.linear_attention(qq, k, v, ld).sum(), qq, create_graph=True)
+        g.sum().backward()
