@@ -395,29 +395,17 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
       for (int e = 0; e < ZE; ++e) if (e0 + ez + e < E) out[e * J.es] = z[e] * unscale;
     }
   } else if (warp < LT_W_OUT) {
-    // ---- scaled v': thread = token s, all in packed bfloat16 arithmetic (fma with one rounding): with the factor
-    // f = f1 + f2 + f3 in bfloat16 parts (24 bits),
-    //   hi = rn(v f1),  m = v f1 - hi (exact),  mid = rn(v f2 + m),  lo = rn(rn(v f2 + (m - mid)) + v f3)
-    // and hi + mid + lo is f v to 2^-23 of it.  Six instructions a pair; splitting the float32 product takes twelve. ----
+    // ---- scaled v': thread = token s; f v is cut into its upper, middle and lower eight bits: three bfloat16 values whose sum is
+    // the float32 product exactly ----
     constexpr int VJ = 8 / LT_VG;                            // 16-byte pieces of a row
     const int s = q * 32 + lane, j0 = ((warp - LT_W_V) >> 2) * VJ;
-    auto split = [&](float f, __nv_bfloat162(&fp)[3]) {
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        const __nv_bfloat16 part = __float2bfloat16_rn(f);
-        fp[i] = __nv_bfloat162(part, part);
-        f -= __bfloat162float(part);
-      }
-    };
     const float fz = local ? J.s_state : J.s_state * zscale;
-    __nv_bfloat162 full[3];
-    split(fz * pw[rev ? s + 1 : LT_T - 1 - s], full);
+    const float f_full = fz * pw[rev ? s + 1 : LT_T - 1 - s];
     const uint32_t row = s * 128u, sw = s & 7u;
 #pragma unroll 1
     for (int c = 0; c < nch; ++c) {
       const int Tv = min(LT_T, s1 - chunk_start(c));
-      __nv_bfloat162 f[3] = {full[0], full[1], full[2]};
-      if (Tv != LT_T) split(s < Tv ? fz * pw[rev ? s + 1 : Tv - 1 - s] : 0.f, f);
+      const float f = Tv == LT_T ? f_full : s < Tv ? fz * pw[rev ? s + 1 : Tv - 1 - s] : 0.f;
       const uint8_t* v = sm + ((c & 1) * LT_STAGE + 4) * BLK;
       uint4 w[VJ];
       bool ok = role_wait(&bars.v_full[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead);
@@ -430,16 +418,21 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
 #pragma unroll
         for (int j = 0; j < VJ; ++j) {
           uint4 oh, om, ol;
-          const __nv_bfloat162* in = reinterpret_cast<const __nv_bfloat162*>(&w[j]);
-          __nv_bfloat162 *ph = reinterpret_cast<__nv_bfloat162*>(&oh), *pm = reinterpret_cast<__nv_bfloat162*>(&om),
-                         *pl = reinterpret_cast<__nv_bfloat162*>(&ol);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 hi = __hmul2_rn(in[i], f[0]), m = __hfma2(in[i], f[0], __hneg2(hi));
-            const __nv_bfloat162 mid = __hfma2(in[i], f[1], m);
-            ph[i] = hi;
-            pm[i] = mid;
-            pl[i] = __hfma2(in[i], f[2], __hfma2(in[i], f[1], __hsub2_rn(m, mid)));
+            float2 y, t;
+            const uint32_t w0 = reinterpret_cast<const uint32_t*>(&w[j])[i];
+            unpack_bf16(w0, y.x, y.y);
+            y = mul2(y, make_float2(f, f));
+            const uint32_t hi = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632);
+            t = make_float2(__uint_as_float(__float_as_uint(y.x) & 0xffff0000u), __uint_as_float(__float_as_uint(y.y) & 0xffff0000u));
+            y = fma2(t, make_float2(-1.f, -1.f), y);
+            const uint32_t mid = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632);
+            t = make_float2(__uint_as_float(__float_as_uint(y.x) & 0xffff0000u), __uint_as_float(__float_as_uint(y.y) & 0xffff0000u));
+            y = fma2(t, make_float2(-1.f, -1.f), y);
+            reinterpret_cast<uint32_t*>(&oh)[i] = hi;
+            reinterpret_cast<uint32_t*>(&om)[i] = mid;
+            reinterpret_cast<uint32_t*>(&ol)[i] = pack_bf16(y.x, y.y);
           }
           uint8_t* dst = sVd + row + (((j0 + j) ^ sw) << 4);
           *reinterpret_cast<uint4*>(dst) = oh;
@@ -511,16 +504,17 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   extern __shared__ uint8_t smem_raw[];
   __shared__ LtShared sh;
   const LaPlan& p = a.p;
-  // tile index: e tile fastest, then job, segment, head, batch
+  // tile index: e tile fastest, then segment, head, batch, and the job last: CTAs that run side by side then share their code
+  // (jobs side by side would share q, k, v and dy in L2, but were 17 % slower in the backward pass)
   int64_t id = blockIdx.x;
   const int ne = p.ne;
   const int et = (int)(id % ne);
   id /= ne;
-  const int jb = (int)(id % p.njobs);
-  id /= p.njobs;
   const int seg = (int)(id % p.nseg);
   id /= p.nseg;
-  const int h = (int)(id % p.H), b = (int)(id / p.H);
+  const int h = (int)(id % p.H);
+  id /= p.H;
+  const int b = (int)(id % p.B), jb = (int)(id / p.B);
   const LaJob& J = p.job[jb];
   const int rev = J.reverse;
   if (et * LT_E >= J.E) return;
