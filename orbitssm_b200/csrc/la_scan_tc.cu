@@ -37,8 +37,7 @@ constexpr int LT_T = 128, LT_E = 64;
 constexpr int LT_ZG = 2, LT_VG = 2;   // groups of four warps for the state and for v'
 constexpr int LT_W_V = 4 + 4 * LT_ZG, LT_W_OUT = LT_W_V + 4 * LT_VG, LT_W_LOAD = LT_W_OUT + 4, LT_THREADS = (LT_W_LOAD + 3) * 32;   // first warps of the roles
 constexpr uint32_t LT_S1 = 0, LT_P = 128, LT_O = 192, LT_DZ = 320;   // TMEM columns: 128, 64, 2 x 64, 192 (512 in all)
-constexpr int LT_STAGE = 5;                                  // blocks of 16 KB: q' 2, k' 2, v' 1
-constexpr int LT_SMEM = (2 * LT_STAGE + 3 + 1) * (int)BLK + 1024;
+constexpr int LT_SMEM = (2 * 5 + 3 + 1) * (int)BLK + 1024;   // two stages of (q' 2, k' 2, v' 1), scaled v' 3, Zb 1 blocks of 16 KB
 constexpr int LT_FWD_C = 64, LT_REV_C = 63;                  // the token that decays are counted from
 
 struct LaTcArgs {
@@ -47,8 +46,8 @@ struct LaTcArgs {
 };
 
 struct LtBars {
-  uint64_t qk_full[2], qk_empty[2], v_full[2], v_empty[2], v_read[2], s1_full, s1_empty, p_full, p_empty, vd_full, vd_empty, zb_full,
-      zb_empty, dz_full, dz_empty, acc_full[2], acc_empty[2];
+  uint64_t qk_full[2], qk_empty[2], v_full[2], v_empty[2], v_read[2], s1_full, s1_empty, p_full, p_empty, vd_full[2], vd_empty[2], zb_full,
+      zb_empty, dz_full[2], dz_empty[2], acc_full[2], acc_empty[2];
 };
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z, int w) {
@@ -97,8 +96,15 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
   const CUtensorMap *mq = &a.map[jb][0], *mk = &a.map[jb][1], *mv = &a.map[jb][2], *my = &a.map[jb][3];
   LtBars& bars = sh.bars;
   const float* pw = sh.pw;
-  uint8_t* sVd = sm + 2 * LT_STAGE * BLK;                    // scaled v': hi, mid, lo
+  // Blocks of a stage and its k' and v' tiles in it.  The state-only launch loads no q' and has room for two sets of scaled v' and
+  // of accumulators, so that scaling, product and state update of three chunks run side by side.
+  constexpr int STAGE = local ? 3 : 5, KO = local ? 0 : 2, VO = local ? 2 : 4, SETS = local ? 2 : 1;
+  uint8_t* sVd = sm + 2 * STAGE * BLK;                       // scaled v': hi, mid, lo
   uint8_t* sZb = sVd + 3 * BLK;                              // entering state, bfloat16 [128 x][64 e]
+  auto set_of = [](int c) { return c % SETS; };
+  auto turn_of = [](int c) { return (uint32_t)((c / SETS) & 1); };   // phase of a set's barriers at chunk c
+  constexpr uint32_t DZ = local ? 0 : LT_DZ;
+  constexpr int VG = local ? 4 : LT_VG;                      // groups that scale v': the mask's and the read-out's warps join there
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3;
   const int s0 = seg * p.seg_len, s1 = min(p.L, s0 + p.seg_len), nch = (s1 - s0 + LT_T - 1) / LT_T;
 
@@ -107,8 +113,12 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
       mbar_init(&bars.qk_full[i], 1);
       mbar_init(&bars.qk_empty[i], local ? 1 : 2);           // released by both issuing warps
       mbar_init(&bars.v_full[i], 1);
-      mbar_init(&bars.v_empty[i], local ? 4 * LT_VG : 1);    // by the read-out, which puts its tile there (local: the scaling warps)
-      mbar_init(&bars.v_read[i], 4 * LT_VG);
+      mbar_init(&bars.v_empty[i], local ? 4 * VG : 1);       // by the read-out, which puts its tile there (local: the scaling warps)
+      mbar_init(&bars.v_read[i], 4 * VG);
+      mbar_init(&bars.vd_full[i], 4 * VG);
+      mbar_init(&bars.vd_empty[i], 1);
+      mbar_init(&bars.dz_full[i], 1);
+      mbar_init(&bars.dz_empty[i], 4 * LT_ZG);
       mbar_init(&bars.acc_full[i], 1);
       mbar_init(&bars.acc_empty[i], 4);
     }
@@ -116,12 +126,8 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
     mbar_init(&bars.s1_empty, 4);
     mbar_init(&bars.p_full, 4);
     mbar_init(&bars.p_empty, 1);
-    mbar_init(&bars.vd_full, 4 * LT_VG);
-    mbar_init(&bars.vd_empty, 1);
     mbar_init(&bars.zb_full, 4 * LT_ZG);
     mbar_init(&bars.zb_empty, 1);
-    mbar_init(&bars.dz_full, 1);
-    mbar_init(&bars.dz_empty, 4 * LT_ZG);
     mbar_fence_init();
     sh.abort_flag = 0;
   }
@@ -141,27 +147,33 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
   if (warp == LT_W_LOAD) {
     if (lane == 0) {
       // ---- producer ----
-      int done = 0;
+      int done_qk = 0, done_v = 0;                           // loads issued
 #pragma unroll 1
       for (int c = 0; c < nch; ++c) {
         const int s = c & 1, t0 = chunk_start(c);
-        uint8_t* st = sm + s * LT_STAGE * BLK;
-        if (c >= 2 && !lane_wait(&bars.qk_empty[s], (uint32_t)(((c >> 1) - 1) & 1), abort_flag, dead)) break;
+        uint8_t* st = sm + s * STAGE * BLK;
         const int blocks = X > 64 ? 2 : 1;                   // the second block of a narrow head is never contracted
+        auto load_v = [&] {
+          if (c >= 2 && !lane_wait(&bars.v_empty[s], (uint32_t)(((c >> 1) - 1) & 1), abort_flag, dead)) return false;
+          mbar_expect_tx(&bars.v_full[s], BLK);
+          tma_load_4d(st + VO * BLK, mv, &bars.v_full[s], e0, h, t0, b);
+          ++done_v;
+          return true;
+        };
+        // whichever place is free first: that of v' where the scaling gives it back, that of q' and k' where the read-out does
+        if (local && !load_v()) break;
+        if (c >= 2 && !lane_wait(&bars.qk_empty[s], (uint32_t)(((c >> 1) - 1) & 1), abort_flag, dead)) break;
         mbar_expect_tx(&bars.qk_full[s], (uint32_t)(local ? blocks : 2 * blocks) * BLK);
         for (int i = 0; i < blocks; ++i) {
           if (!local) tma_load_4d(st + i * BLK, mq, &bars.qk_full[s], i * 64, h, t0, b);
-          tma_load_4d(st + (2 + i) * BLK, mk, &bars.qk_full[s], i * 64, h, t0, b);
+          tma_load_4d(st + (KO + i) * BLK, mk, &bars.qk_full[s], i * 64, h, t0, b);
         }
-        done = 2 * c + 1;
-        if (c >= 2 && !lane_wait(&bars.v_empty[s], (uint32_t)(((c >> 1) - 1) & 1), abort_flag, dead)) break;
-        mbar_expect_tx(&bars.v_full[s], BLK);
-        tma_load_4d(st + 4 * BLK, mv, &bars.v_full[s], e0, h, t0, b);
-        done = 2 * c + 2;
+        ++done_qk;
+        if (!local && !load_v()) break;
       }
       if (dead) {                                            // wind-down: what was issued has to land before the CTA goes
-        for (int k = max(0, done - 4); k < done; ++k)
-          mbar_wait((k & 1) ? &bars.v_full[(k >> 1) & 1] : &bars.qk_full[(k >> 1) & 1], (uint32_t)((k >> 2) & 1));
+        for (int k = max(0, done_qk - 2); k < done_qk; ++k) mbar_wait(&bars.qk_full[k & 1], (uint32_t)((k >> 1) & 1));
+        for (int k = max(0, done_v - 2); k < done_v; ++k) mbar_wait(&bars.v_full[k & 1], (uint32_t)((k >> 1) & 1));
       }
     }
     __syncwarp();
@@ -171,9 +183,9 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
       const uint32_t id_s = idesc_bf16(128, 128, 0, 0), id_o = idesc_bf16(128, 64, 0, 1);
       const int kx = (X + 15) / 16;
       const uint32_t zb = lo_mn(smem_u32(sZb));
-      auto base = [&](int c, int blk) { return smem_u32(sm + ((c & 1) * LT_STAGE + blk) * BLK); };
+      auto base = [&](int c, int blk) { return smem_u32(sm + ((c & 1) * STAGE + blk) * BLK); };
       auto scores = [&](int c) {
-        const uint32_t aq = lo_k(base(c, 0)), bk = lo_k(base(c, 2));
+        const uint32_t aq = lo_k(base(c, 0)), bk = lo_k(base(c, KO));
         if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
@@ -211,7 +223,7 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
         if (!role_wait(&bars.p_full, ph, abort_flag, dead)) break;
         if (!role_wait(&bars.v_full[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead)) break;
         tc_fence_after_sync();
-        const uint32_t bv = lo_mn(base(c, 4));
+        const uint32_t bv = lo_mn(base(c, VO));
         if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
@@ -228,21 +240,22 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
 #pragma unroll 1
     for (int c = 0; c < nch && !dead; ++c) {
       if (!role_wait(&bars.qk_full[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead)) break;
-      if (c > 0 && !role_wait(&bars.dz_empty, (uint32_t)((c - 1) & 1), abort_flag, dead)) break;
-      if (!role_wait(&bars.vd_full, (uint32_t)(c & 1), abort_flag, dead)) break;
+      const int set = set_of(c);
+      if (c >= SETS && !role_wait(&bars.dz_empty[set], turn_of(c - SETS), abort_flag, dead)) break;
+      if (!role_wait(&bars.vd_full[set], turn_of(c), abort_flag, dead)) break;
       tc_fence_after_sync();
-      const uint32_t ak = lo_mn(smem_u32(sm + ((c & 1) * LT_STAGE + 2) * BLK));
+      const uint32_t ak = lo_mn(smem_u32(sm + ((c & 1) * STAGE + KO) * BLK));
       if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) umma_bf16_h(tbase + LT_DZ, ak + inc_mn(ks), vd + inc_mn(ks), id_z, ks > 0 ? 1u : 0u);
-        umma_commit(&bars.dz_full);
-        umma_commit(&bars.vd_empty);
+        for (int ks = 0; ks < 8; ++ks) umma_bf16_h(tbase + DZ + set * 192, ak + inc_mn(ks), vd + set * ((3 * BLK) >> 4) + inc_mn(ks), id_z, ks > 0 ? 1u : 0u);
+        umma_commit(&bars.dz_full[set]);
+        umma_commit(&bars.vd_empty[set]);
         umma_commit(&bars.qk_empty[c & 1]);
       }
     }
     __syncwarp();
-  } else if (warp < 4) {
-    if (!local) {
+  } else if (!local && warp < 4) {
+    {
       // ---- decay mask: thread = row t; slab j holds columns 32 j .. 32 j + 31 ----
       {
         uint32_t z[16];
@@ -307,7 +320,7 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
         if (lane == 0) mbar_arrive(&bars.p_full);
       }
     }
-  } else if (warp < LT_W_V) {
+  } else if (warp >= 4 && warp < LT_W_V) {
     // ---- state: thread = state row x, ZE of its channels in registers ----
     constexpr int ZE = LT_E / LT_ZG;
     const int hf = (warp - 4) >> 2, ez = hf * ZE;            // first of this thread's channels in the tile
@@ -367,14 +380,16 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
         warp_arrive(&bars.zb_full, true);
       }
       const float aT = Tv == LT_T ? a_full : pw[Tv];
-      if (role_wait(&bars.dz_full, (uint32_t)(c & 1), abort_flag, dead)) {
+      const int set = set_of(c);
+      if (role_wait(&bars.dz_full[set], turn_of(c), abort_flag, dead)) {
         tc_fence_after_sync();
+        const uint32_t dz = tmem_addr(tbase, q * 32, DZ + set * 192 + ez);
 #pragma unroll
         for (int j = 0; j < ZE / 8; ++j) {
           uint32_t hi[8], mi[8], lo[8];
-          tmem_ld8(tmem_addr(tbase, q * 32, LT_DZ + ez + j * 8), hi);
-          tmem_ld8(tmem_addr(tbase, q * 32, LT_DZ + 64 + ez + j * 8), mi);
-          tmem_ld8(tmem_addr(tbase, q * 32, LT_DZ + 128 + ez + j * 8), lo);
+          tmem_ld8(dz + j * 8, hi);
+          tmem_ld8(dz + 64 + j * 8, mi);
+          tmem_ld8(dz + 128 + j * 8, lo);
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 8; i += 2) {
@@ -385,7 +400,7 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
           }
         }
       }
-      warp_arrive(&bars.dz_empty, false);
+      warp_arrive(&bars.dz_empty[set], false);
     }
     float* out = local ? J.part + (head * p.nseg + seg) * p.S : (J.z1 && seg == (rev ? 0 : p.nseg - 1) ? J.z1 + head * p.S : nullptr);
     if (out && live && !dead) {
@@ -394,11 +409,12 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
 #pragma unroll
       for (int e = 0; e < ZE; ++e) if (e0 + ez + e < E) out[e * J.es] = z[e] * unscale;
     }
-  } else if (warp < LT_W_OUT) {
+  } else if (local || (warp >= LT_W_V && warp < LT_W_OUT)) {
     // ---- scaled v': thread = token s; f v is cut into its upper, middle and lower eight bits: three bfloat16 values whose sum is
     // the float32 product exactly ----
-    constexpr int VJ = 8 / LT_VG;                            // 16-byte pieces of a row
-    const int s = q * 32 + lane, j0 = ((warp - LT_W_V) >> 2) * VJ;
+    constexpr int VJ = 8 / VG;                               // 16-byte pieces of a row
+    const int g = warp >= LT_W_OUT ? 3 : warp >= LT_W_V ? (warp - LT_W_V) >> 2 : 2;
+    const int s = q * 32 + lane, j0 = g * VJ;
     const float fz = local ? J.s_state : J.s_state * zscale;
     const float f_full = fz * pw[rev ? s + 1 : LT_T - 1 - s];
     const uint32_t row = s * 128u, sw = s & 7u;
@@ -406,14 +422,19 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
     for (int c = 0; c < nch; ++c) {
       const int Tv = min(LT_T, s1 - chunk_start(c));
       const float f = Tv == LT_T ? f_full : s < Tv ? fz * pw[rev ? s + 1 : Tv - 1 - s] : 0.f;
-      const uint8_t* v = sm + ((c & 1) * LT_STAGE + 4) * BLK;
+      const uint8_t* v = sm + ((c & 1) * STAGE + VO) * BLK;
       uint4 w[VJ];
       bool ok = role_wait(&bars.v_full[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead);
       if (ok) {
 #pragma unroll
         for (int j = 0; j < VJ; ++j) w[j] = *reinterpret_cast<const uint4*>(v + row + (((j0 + j) ^ sw) << 4));   // all of them before the first store
       }
-      if (c > 0) ok = role_wait(&bars.vd_empty, (uint32_t)((c - 1) & 1), abort_flag, dead) && ok;
+      if (local) {                                           // nothing else reads the v' tile there
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.v_empty[c & 1]);
+      }
+      const int set = set_of(c);
+      if (c >= SETS) ok = role_wait(&bars.vd_empty[set], turn_of(c - SETS), abort_flag, dead) && ok;
       if (ok) {
 #pragma unroll
         for (int j = 0; j < VJ; ++j) {
@@ -434,23 +455,23 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
             reinterpret_cast<uint32_t*>(&om)[i] = mid;
             reinterpret_cast<uint32_t*>(&ol)[i] = pack_bf16(y.x, y.y);
           }
-          uint8_t* dst = sVd + row + (((j0 + j) ^ sw) << 4);
+          uint8_t* dst = sVd + set * 3 * BLK + row + (((j0 + j) ^ sw) << 4);
           *reinterpret_cast<uint4*>(dst) = oh;
           *reinterpret_cast<uint4*>(dst + BLK) = om;
           *reinterpret_cast<uint4*>(dst + 2 * BLK) = ol;
         }
       }
-      warp_arrive(&bars.vd_full, true);                      // ends in a warp barrier: every lane has read its part of v'
-      if (lane == 0) mbar_arrive(local ? &bars.v_empty[c & 1] : &bars.v_read[c & 1]);
+      warp_arrive(&bars.vd_full[set], true);                     // ends in a warp barrier: every lane has read its part of v'
+      if (!local && lane == 0) mbar_arrive(&bars.v_read[c & 1]);
     }
-  } else if (!local && warp < LT_W_LOAD) {
+  } else if (warp < LT_W_LOAD) {
     // ---- read-out: thread = row t; the tile leaves from the place of the v' tile ----
     const int t = q * 32 + lane;
     const float fo = J.s_out * (steep ? 1.f : power(pw, rev ? LT_REV_C - t : t - LT_FWD_C));   // row factor
 #pragma unroll 1
     for (int c = 0; c < nch; ++c) {
       const int t0 = chunk_start(c), Tv = min(LT_T, s1 - t0);
-      uint8_t* out = sm + ((c & 1) * LT_STAGE + 4) * BLK;
+      uint8_t* out = sm + ((c & 1) * STAGE + VO) * BLK;
       bool ok = role_wait(&bars.acc_full[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead);   // the product has read the v' tile ...
       ok = role_wait(&bars.v_read[c & 1], (uint32_t)((c >> 1) & 1), abort_flag, dead) && ok;    // ... and so has the scaling
       if (ok) {
@@ -504,16 +525,16 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   extern __shared__ uint8_t smem_raw[];
   __shared__ LtShared sh;
   const LaPlan& p = a.p;
-  // tile index: e tile fastest, then segment, head, batch, and the job last: CTAs that run side by side then share their code
+  // tile index: e tile fastest, then head (neighbours in memory), segment, batch, and the job last: CTAs that run side by side then share their code
   // (jobs side by side would share q, k, v and dy in L2, but were 17 % slower in the backward pass)
   int64_t id = blockIdx.x;
   const int ne = p.ne;
   const int et = (int)(id % ne);
   id /= ne;
-  const int seg = (int)(id % p.nseg);
-  id /= p.nseg;
   const int h = (int)(id % p.H);
   id /= p.H;
+  const int seg = (int)(id % p.nseg);
+  id /= p.nseg;
   const int b = (int)(id % p.B), jb = (int)(id / p.B);
   const LaJob& J = p.job[jb];
   const int rev = J.reverse;
