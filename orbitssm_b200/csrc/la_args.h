@@ -28,7 +28,7 @@ struct LaJob {
 };
 struct LaPlan {
   int B, L, H, S;     // S = Dk * Dv, elements of a head's state
-  int njobs, nseg, seg_len, ne;   // ne: tiles of output channels (tensor-core launch)
+  int njobs, nseg, seg_len, ne;   // ne: CTAs that share a head's channels (tensor-core launch)
   const float* log_decay;
   int* status;
   LaJob job[3];
@@ -37,7 +37,7 @@ struct LaPlan {
 // the jobs of one direction (local: the two state-only passes that feed `part`)
 int la_plan(const LaArgs& a, bool bwd, int nseg, int seg_len, bool local, LaPlan* p);
 // segments the sequence is split into so that `units` CTAs per segment fill the GPU (chunk = tokens of one tile)
-int la_segments(int64_t units, int L, int chunk, int* seg_len);
+int la_segments(int64_t units, int L, int chunk, int* seg_len, double* cost = nullptr);
 
 bool la_tc_serves(const LaArgs& a, bool bwd, int dtype);
 int la_tc_launch(const LaArgs& a, bool bwd, cudaStream_t st);

@@ -285,7 +285,7 @@ int la_plan(const LaArgs& a, bool bwd, int nseg, int seg_len, bool local, LaPlan
 // The split that takes the fewest chunk steps on 148 SMs: rounds of CTAs times the chunks of a segment, and for more than one
 // segment the first launch, which reads half of the operands and costs about half a step.  At most 32 segments, so that the
 // sum over the earlier ones stays small against a segment's walk.
-int la_segments(int64_t units, int L, int chunk, int* seg_len) {
+int la_segments(int64_t units, int L, int chunk, int* seg_len, double* cost_out) {
   const int nch = (L + chunk - 1) / chunk;
   int best = 1, best_len = nch;
   double best_cost = 0.;
@@ -298,6 +298,7 @@ int la_segments(int64_t units, int L, int chunk, int* seg_len) {
     if (n == 1 || cost < 0.95 * best_cost) { best = n; best_len = per; best_cost = cost; }
   }
   *seg_len = best_len * chunk;
+  if (cost_out) *cost_out = best_cost;
   return best;
 }
 
