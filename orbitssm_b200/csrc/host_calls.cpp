@@ -163,7 +163,7 @@ PyObject* la_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.workspace = ws.data_ptr();
     }
     const int rc = entry.la_fwd(&p, code, stream(dev));
-    return result(rc, y, s1, p.workspace_bytes ? 2 : 1);
+    return result(rc, y, s1, p.workspace_bytes ? 3 : 1);
   })
 }
 
@@ -212,7 +212,7 @@ PyObject* la_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const int rc = entry.la_bwd(&p, code, stream(dev));
     PyObject* o[6] = {THPVariable_Wrap(dq), THPVariable_Wrap(dk), THPVariable_Wrap(dv), ds0.defined() ? THPVariable_Wrap(ds0) : Py_NewRef(Py_None),
-                      PyLong_FromLong(rc), PyLong_FromLong(p.workspace_bytes ? 2 : 1)};
+                      PyLong_FromLong(rc), PyLong_FromLong(p.workspace_bytes ? 3 : 1)};
     PyObject* out = o[0] && o[1] && o[2] && o[3] && o[4] && o[5] ? PyTuple_Pack(6, o[0], o[1], o[2], o[3], o[4], o[5]) : nullptr;
     for (PyObject* x : o) Py_XDECREF(x);
     return out;

@@ -23,7 +23,8 @@ struct LaJob {
   float s_out, s_in, s_state;
   const float* z0;    // state before the sequence (reverse: gradient of the state after it) or null
   float* z1;          // state after it (reverse: gradient of the state before it) or null
-  float* part;        // [B*H][nseg][Dv*Dk]: what each segment alone adds to the state, null when nseg == 1
+  float* part;        // [B*H][nseg][Dv*Dk]: what each segment alone adds to the state, then (joined) the state that enters each
+                      // segment; null when nseg == 1
   int64_t xs, es;
 };
 struct LaPlan {
@@ -36,6 +37,8 @@ struct LaPlan {
 
 // the jobs of one direction (local: the two state-only passes that feed `part`)
 int la_plan(const LaArgs& a, bool bwd, int nseg, int seg_len, bool local, LaPlan* p);
+// the launch between the two: shares of the segments -> states that enter them, in place, for the jobs of the state-only plan
+int la_join(const LaPlan& p, cudaStream_t st);
 // segments the sequence is split into so that `units` CTAs per segment fill the GPU (chunk = tokens of one tile)
 int la_segments(int64_t units, int L, int chunk, int* seg_len, double* cost = nullptr);
 

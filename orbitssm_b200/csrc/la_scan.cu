@@ -10,8 +10,8 @@
 // the chunk, so the row factor is a^{T-1-t} and the write factor a^{s+1}.
 //
 // Few (batch, head) pairs and a long sequence: the sequence is split into segments.  A first launch forms what each segment
-// alone adds to the state; each CTA of the second launch sums the earlier segments' shares for its own entering state (at most
-// 31 reads of its tile) and walks its segment.  No CTA waits on another.
+// alone adds to the state, a second joins these shares into the states that enter the segments, and each CTA of the third walks
+// its segment from there.  No CTA waits on another.
 //
 // One CTA of 256 threads owns a head's segment and 64 output channels; 4 x 4 register tiles (float4 reads of operands that
 // are kept transposed in shared memory).  Bound by the FP32 pipe and shared-memory reads.
@@ -59,24 +59,11 @@ __global__ void __launch_bounds__(LG_THREADS) la_generic_kernel(const __grid_con
 
   const int s0 = seg * p.seg_len, s1 = min(p.L, s0 + p.seg_len);
   const int64_t head = (int64_t)b * p.H + h;
-  // entering state: the carried one and the shares of the segments before this one, each with its decay since
+  // the state that enters the segment (joined from the segments' shares, or the carried one)
+  const float* enter = local ? nullptr : J.part ? J.part + (head * p.nseg + seg) * p.S : J.z0 ? J.z0 + head * p.S : nullptr;
   for (int i = tid; i < X4 * LG_E; i += LG_THREADS) {
     const int e = J.xs == 1 ? i / X4 : i % LG_E, x = J.xs == 1 ? i % X4 : i / LG_E;   // the axis that lies dense goes along threads
-    float z = 0.f;
-    if (!local && x < X && e0 + e < E) {
-      const int64_t off = x * J.xs + (e0 + e) * J.es;
-      if (J.z0) z = J.z0[head * p.S + off];
-      if (J.part) {
-        const float full = (float)exp(ld * p.seg_len);
-        if (!rev) {
-          for (int s = 0; s < seg; ++s) z = fmaf(full, z, J.part[(head * p.nseg + s) * p.S + off]);
-        } else {
-          for (int s = p.nseg - 1; s > seg; --s)
-            z = fmaf(s == p.nseg - 1 ? (float)exp(ld * (p.L - s * p.seg_len)) : full, z, J.part[(head * p.nseg + s) * p.S + off]);
-        }
-      }
-    }
-    Z[x * LG_E + e] = z;
+    Z[x * LG_E + e] = enter && x < X && e0 + e < E ? enter[x * J.xs + (e0 + e) * J.es] : 0.f;
   }
 
   const IO* q = (const IO*)J.q + b * J.q_bs + h * J.q_hs;
@@ -224,6 +211,34 @@ __global__ void __launch_bounds__(LG_THREADS) la_generic_kernel(const __grid_con
   }
 }
 
+// One thread an element of a head's state: walks the segments in the direction's order, in place.
+__global__ void __launch_bounds__(256) la_join_kernel(const __grid_constant__ LaPlan p) {
+  const LaJob& J = p.job[blockIdx.y];
+  const int blocks = (p.S + 255) / 256, rev = J.reverse, n = p.nseg;
+  const int i = (int)(blockIdx.x % blocks) * 256 + threadIdx.x;
+  const int64_t head = blockIdx.x / blocks;
+  if (i >= p.S) return;
+  const double ld = (double)p.log_decay[head % p.H];
+  const float full = (float)exp(ld * p.seg_len), last = (float)exp(ld * (p.L - (n - 1) * p.seg_len));
+  float* part = J.part + head * n * p.S + i;
+  float z = J.z0 ? J.z0[head * p.S + i] : 0.f;
+#pragma unroll 4
+  for (int k = 0; k < n; ++k) {
+    const int s = rev ? n - 1 - k : k;
+    const float share = k < n - 1 ? part[(int64_t)s * p.S] : 0.f;          // nobody formed the last one's
+    part[(int64_t)s * p.S] = z;
+    z = fmaf(s == n - 1 ? last : full, z, share);
+  }
+}
+
+int la_join(const LaPlan& p, cudaStream_t st) {
+  const int64_t grid = (int64_t)p.B * p.H * ((p.S + 255) / 256);
+  ORBIT_REQUIRE(grid <= 0x7fffffffLL, ERR_UNSUPPORTED, "orbit_la: %lld (batch, head) states are too many for one call", (long long)p.B * p.H);
+  la_join_kernel<<<dim3((unsigned)grid, p.njobs), 256, 0, st>>>(p);
+  ORBIT_CHECK_LAUNCH("la_join_kernel");
+  return OK;
+}
+
 int la_plan(const LaArgs& a, bool bwd, int nseg, int seg_len, bool local, LaPlan* p) {
   *p = LaPlan{};
   p->B = a.B; p->L = a.L; p->H = a.H; p->S = a.Dk * a.Dv;
@@ -282,9 +297,9 @@ int la_plan(const LaArgs& a, bool bwd, int nseg, int seg_len, bool local, LaPlan
   return OK;
 }
 
-// The split that takes the fewest chunk steps on 148 SMs: rounds of CTAs times the chunks of a segment, and for more than one
-// segment the first launch, which reads half of the operands and costs about half a step.  At most 32 segments, so that the
-// sum over the earlier ones stays small against a segment's walk.
+// The split that takes the fewest chunk steps on 148 SMs: rounds of CTAs times the chunks of a segment and three steps' worth of
+// set-up; for more than one segment also the first launch, which reads half of the operands and costs about half a step for each,
+// and the join, about two steps.  At most 32 segments: more would only fill rounds that are full.
 int la_segments(int64_t units, int L, int chunk, int* seg_len, double* cost_out) {
   const int nch = (L + chunk - 1) / chunk;
   int best = 1, best_len = nch;
@@ -293,8 +308,7 @@ int la_segments(int64_t units, int L, int chunk, int* seg_len, double* cost_out)
     const int per = (nch + n - 1) / n, ns = (nch + per - 1) / per;
     if (ns != n) continue;
     const int64_t rounds = (units * n + 147) / 148, first = (units * (n - 1) + 147) / 148;
-    // a segment more costs each CTA one more read of its state tile: a twentieth of a chunk step
-    const double cost = (double)rounds * (per + 1) + (n > 1 ? 0.5 * (double)first * (per + 1) + 0.05 * n : 0.);
+    const double cost = (double)rounds * (per + 3) + (n > 1 ? 0.5 * (double)first * (per + 3) + 2. : 0.);
     if (n == 1 || cost < 0.95 * best_cost) { best = n; best_len = per; best_cost = cost; }
   }
   *seg_len = best_len * chunk;
@@ -331,6 +345,7 @@ static int lg_run(const LaArgs& a, bool bwd, int dtype, cudaStream_t st) {
     if ((rc = la_plan(a, bwd, nseg, seg_len, local != 0, &p)) != OK) return rc;
     if (dtype == BF16) rc = T == 64 ? lg_launch<__nv_bfloat16, 64>(p, local, st) : lg_launch<__nv_bfloat16, 32>(p, local, st);
     else rc = T == 64 ? lg_launch<float, 64>(p, local, st) : lg_launch<float, 32>(p, local, st);
+    if (rc == OK && local) rc = la_join(p, st);
     if (rc != OK) return rc;
   }
   return OK;
@@ -376,6 +391,11 @@ extern "C" int orbit_la_fwd(const orbit_la_args* a, int dtype, void* stream) {
     return OK;
   }
   ORBIT_REQUIRE(a->q && a->k && a->v && a->y && a->log_decay, ERR_BAD_ARG, "orbit_la_fwd: null q/k/v/y/log_decay");
+  // One token with a state on either side is the decode step: its kernel takes a third of the time of a tile with one row (at 16
+  // heads of 128 x 128: 5 us against 14).
+  if (a->L == 1 && a->state0 && a->state1 && (a->H == 1 || a->y_hs == a->Dv) && (a->B == 1 || a->y_bs == (int64_t)a->H * a->Dv))
+    return orbit_la_step(a->q, a->q_bs, a->q_hs, a->k, a->k_bs, a->k_hs, a->v, a->v_bs, a->v_hs, a->log_decay, a->state0, a->state1, a->y,
+                         a->B, a->H, a->Dk, a->Dv, a->scale, dtype, stream);
   return la_run(a, false, dtype, stream, "orbit_la_fwd");
 }
 

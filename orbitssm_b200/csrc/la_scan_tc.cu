@@ -135,6 +135,12 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
   auto dz_turn = [](int c) { return (uint32_t)((c / SETS) & 1); };
   auto chunk_start = [&](int c) { return s0 + (rev ? nch - 1 - c : c) * LT_T; };
 
+  if (tid == LT_THREADS - 1) {                               // the descriptors' first fetch, under the rest of the set-up
+    if (!local) tma_prefetch_desc(mq);
+    tma_prefetch_desc(mk);
+    tma_prefetch_desc(mv);
+    if (!local) tma_prefetch_desc(my);
+  }
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.qk_full[i], 1);
@@ -365,31 +371,20 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
     for (int x = 0; x < ZX; ++x) z[x] = 0.f;
     const bool live = e < E && x0 < X;
     if (!local && live) {
-      // the carried state and the shares of the segments before this one, each with its decay since
-      const int64_t off = x0 * J.xs + (e0 + e) * J.es;
-      // z = f z + a share; where a thread's 64 values lie side by side (xs = 1) in float4s, X and the strides being multiples of 8
-      auto add = [&](const float* src, float f) {
-        if (J.xs == 1 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+      // the state that enters the segment (joined from the segments' shares, or the carried one)
+      const float* src = J.part ? J.part + (head * p.nseg + seg) * p.S : J.z0 ? J.z0 + head * p.S : nullptr;
+      if (src) {
+        src += x0 * J.xs + (e0 + e) * J.es;
+        if (J.xs == 1 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {       // 64 values side by side; X is a multiple of 8
 #pragma unroll
           for (int x = 0; x < ZX; x += 4)
             if (x0 + x < X) {
               const float4 w = *reinterpret_cast<const float4*>(src + x);
-              z[x] = fmaf(f, z[x], w.x); z[x + 1] = fmaf(f, z[x + 1], w.y); z[x + 2] = fmaf(f, z[x + 2], w.z); z[x + 3] = fmaf(f, z[x + 3], w.w);
+              z[x] = w.x; z[x + 1] = w.y; z[x + 2] = w.z; z[x + 3] = w.w;
             }
         } else {
 #pragma unroll
-          for (int x = 0; x < ZX; ++x) if (x0 + x < X) z[x] = fmaf(f, z[x], src[x * J.xs]);
-        }
-      };
-      if (J.z0) add(J.z0 + head * p.S + off, 0.f);
-      if (J.part) {
-        const float full = (float)exp(ld * p.seg_len);
-        const int n = rev ? p.nseg - 1 - seg : seg;
-#pragma unroll 1
-        for (int i = 0; i < n; ++i) {
-          const int s = rev ? p.nseg - 1 - i : i;
-          const float f = s == p.nseg - 1 ? (float)exp(ld * (p.L - s * p.seg_len)) : full;
-          add(J.part + (head * p.nseg + s) * p.S + off, f);
+          for (int x = 0; x < ZX; ++x) if (x0 + x < X) z[x] = src[x * J.xs];
         }
       }
     }
@@ -444,8 +439,14 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
     if (out && live && !dead) {
       out += x0 * J.xs + (e0 + e) * J.es;
       const float unscale = 1.f / zscale;
+      if (J.xs == 1 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
 #pragma unroll
-      for (int x = 0; x < ZX; ++x) if (x0 + x < X) out[x * J.xs] = z[x] * unscale;
+        for (int x = 0; x < ZX; x += 4)
+          if (x0 + x < X) *reinterpret_cast<float4*>(out + x) = make_float4(z[x] * unscale, z[x + 1] * unscale, z[x + 2] * unscale, z[x + 3] * unscale);
+      } else {
+#pragma unroll
+        for (int x = 0; x < ZX; ++x) if (x0 + x < X) out[x * J.xs] = z[x] * unscale;
+      }
     }
   } else if (warp < LT_W_OUT) {
     regs_dec<LT_R_V>();
@@ -686,6 +687,7 @@ int la_tc_launch(const LaArgs& a, bool bwd, cudaStream_t st) {
     ORBIT_REQUIRE(grid <= 0x7fffffffLL, ERR_UNSUPPORTED, "orbit_la: %lld (batch, head, segment) tiles are too many for one call", (long long)grid);
     la_tc_kernel<<<(unsigned)grid, LT_THREADS, LT_SMEM, st>>>(t, local);
     ORBIT_CHECK_LAUNCH("la_tc_kernel");
+    if (local && (rc = la_join(t.p, st)) != OK) return rc;
   }
   return OK;
 }

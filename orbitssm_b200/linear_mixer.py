@@ -85,7 +85,7 @@ def _run(name, fn, bwd, q, k, v, log_decay, state, scale, code, tail):
         nbytes = lib.orbit_la_workspace_bytes(_PACK.pack(*fields, 0, 0, status), bwd, code)
         if nbytes:
             ws = torch.empty((nbytes,), device=dev, dtype=torch.uint8)
-    launch(name, 1 if ws is None else 2, dev, fn, _PACK.pack(*fields, 0 if ws is None else ws.data_ptr(), nbytes, status), code)
+    launch(name, 1 if ws is None else 3, dev, fn, _PACK.pack(*fields, 0 if ws is None else ws.data_ptr(), nbytes, status), code)
 
 
 def la_fwd(q, k, v, log_decay, state, scale, want_state):
