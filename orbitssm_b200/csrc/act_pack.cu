@@ -11,7 +11,8 @@
 // most).  A non-finite element takes the code -128, which nothing else uses, and is restored as NaN; it does not enter amax, so its
 // neighbours keep their precision.
 //
-// HBM-bound: es + 1 + 1/32 bytes an element in either direction; 16-byte accesses on both sides where rows allow.
+// HBM-bound: es + 1 + 1/32 bytes an element in either direction; 16-byte accesses on both sides where rows allow.  Both directions
+// of 67 million elements in rows of 1024: bfloat16 72 us (5.6 TB/s), float32 131 us (5.1 TB/s).
 #include "common.cuh"
 #include "../../include/orbit_b200.h"
 
@@ -155,76 +156,169 @@ __global__ void __launch_bounds__(PACK_THREADS) unpack_flat_kernel(const uint4* 
   }
 }
 
-// Any width, any row stride: eight lanes own a group, four elements each (one 4-element access where `vec` says that the rows
-// allow it).  Every lane of a warp takes part in the shuffles; the ones past the end hold nothing.
-template <typename T>
-__global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const T* __restrict__ x, int64_t xrs, uint8_t* __restrict__ q,
-                                                                 uint8_t* __restrict__ e, int64_t M, int D, int G, int vec) {
-  const int64_t gid = ((int64_t)blockIdx.x * PACK_THREADS + threadIdx.x) >> 3;
-  const int sub = threadIdx.x & 7;
-  const bool live = gid < M * G;
-  const int64_t row = live ? gid / G : 0;
-  const int c = live ? (int)(gid - row * G) * PACK_GROUP + sub * 4 : D;
-  float f[4] = {0.f, 0.f, 0.f, 0.f};
-  if (c < D) {
-    const T* p = x + row * xrs + c;
-    if (vec) {
-      if constexpr (sizeof(T) == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        unpack_bf16(u.x, f[0], f[1]);
-        unpack_bf16(u.y, f[2], f[3]);
-      } else {
-        const float4 u = *reinterpret_cast<const float4*>(p);
-        f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) if (c + j < D) f[j] = ldf(p + j);
-    }
+// Any width, any row stride: four lanes own a group, eight elements each, in accesses of W elements (8, 4, 2 or 1: what the width,
+// the row stride and the addresses allow) that the lanes take in turn, so that one access of the four lies side by side.  ROW_ITEMS groups a lane in flight.  Both directions of 67 million bfloat16
+// elements in rows of 1000: 91 us (4.5 TB/s; eight lanes of four elements took 109), of 250: 115 us; odd widths move single
+// bytes: 203 us in rows of 251.  Every lane of a warp takes part in the shuffles;
+// the ones past the end hold nothing.
+constexpr int ROW_ITEMS = 2, LANE_ELEMS = 8, GROUP_LANES = PACK_GROUP / LANE_ELEMS;
+constexpr int ROW_GROUPS = PACK_THREADS / GROUP_LANES;                 // groups a block and item
+
+// n / d for n < 2^31 without a division: (high word of n m, plus n) >> s
+struct FastDiv {
+  uint32_t d, m, s;
+  explicit FastDiv(uint32_t d_) : d(d_), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
   }
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) m = max(m, finite_abs_bits(f[j]));
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (!live) return;
-  const uint32_t b = group_exponent(m);
-  if (sub == 0) e[gid] = (uint8_t)b;
-  if (c >= D) return;
-  const float inv = inv_scale(b);
-  if (b == TOP_EXPONENT) keep_finite(f);
-  const uint32_t w = pack4(code_of(f[0], inv), code_of(f[1], inv), code_of(f[2], inv), code_of(f[3], inv));
-  uint8_t* d = q + row * D + c;
-  if (vec) {
-    *reinterpret_cast<uint32_t*>(d) = w;
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
+// W elements between memory and registers in the widest accesses (16 bytes at most)
+template <int W> __device__ __forceinline__ void load_w(const __nv_bfloat16* p, float* f) {
+  if constexpr (W == 8) {
+    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+    unpack_bf16(u.x, f[0], f[1]);
+    unpack_bf16(u.y, f[2], f[3]);
+    unpack_bf16(u.z, f[4], f[5]);
+    unpack_bf16(u.w, f[6], f[7]);
+  } else if constexpr (W == 4) {
+    const uint2 u = __ldcs(reinterpret_cast<const uint2*>(p));
+    unpack_bf16(u.x, f[0], f[1]);
+    unpack_bf16(u.y, f[2], f[3]);
+  } else if constexpr (W == 2) {
+    unpack_bf16(__ldcs(reinterpret_cast<const uint32_t*>(p)), f[0], f[1]);
   } else {
+    f[0] = ldf(p);
+  }
+}
+template <int W> __device__ __forceinline__ void load_w(const float* p, float* f) {
+  if constexpr (W >= 4) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) if (c + j < D) d[j] = (uint8_t)(w >> (8 * j));
+    for (int i = 0; i < W; i += 4) {
+      const float4 u = __ldcs(reinterpret_cast<const float4*>(p + i));
+      f[i] = u.x; f[i + 1] = u.y; f[i + 2] = u.z; f[i + 3] = u.w;
+    }
+  } else if constexpr (W == 2) {
+    const float2 u = __ldcs(reinterpret_cast<const float2*>(p));
+    f[0] = u.x; f[1] = u.y;
+  } else {
+    f[0] = __ldcs(p);
+  }
+}
+template <int W> __device__ __forceinline__ void store_w(__nv_bfloat16* p, const float* f) {
+  if constexpr (W == 8)
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])));
+  else if constexpr (W == 4) __stcs(reinterpret_cast<uint2*>(p), make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3])));
+  else if constexpr (W == 2) __stcs(reinterpret_cast<uint32_t*>(p), pack_bf16(f[0], f[1]));
+  else stf(p, f[0]);
+}
+template <int W> __device__ __forceinline__ void store_w(float* p, const float* f) {
+  if constexpr (W >= 4) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) __stcs(reinterpret_cast<float4*>(p + i), make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]));
+  } else if constexpr (W == 2) __stcs(reinterpret_cast<float2*>(p), make_float2(f[0], f[1]));
+  else __stcs(p, f[0]);
+}
+// bytes j .. j + W - 1 of the eight codes in w
+template <int W> __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t (&w)[2], int j) {
+  if constexpr (W == 8) __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
+  else if constexpr (W == 4) __stcs(reinterpret_cast<uint32_t*>(p), w[j >> 2]);
+  else if constexpr (W == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)(w[j >> 2] >> (8 * (j & 3)));
+  else *p = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+}
+template <int W> __device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t (&w)[2], int j) {
+  if constexpr (W == 8) {
+    const uint2 u = __ldcs(reinterpret_cast<const uint2*>(p));
+    w[0] = u.x; w[1] = u.y;
+  } else if constexpr (W == 4) w[j >> 2] = __ldcs(reinterpret_cast<const uint32_t*>(p));
+  else if constexpr (W == 2) w[j >> 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(p) << (8 * (j & 3));
+  else w[j >> 2] |= (uint32_t)*p << (8 * (j & 3));
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const T* __restrict__ x, int64_t xrs, uint8_t* __restrict__ q,
+                                                                 uint8_t* __restrict__ e, uint32_t groups, int D, const FastDiv G) {
+  const int sub = threadIdx.x % GROUP_LANES;
+  const uint32_t first = blockIdx.x * (ROW_ITEMS * ROW_GROUPS) + threadIdx.x / GROUP_LANES;
+  float f[ROW_ITEMS][LANE_ELEMS];
+#pragma unroll
+  for (int i = 0; i < ROW_ITEMS; ++i) {
+    const uint32_t gid = first + i * ROW_GROUPS, row = G.quotient(gid);
+    const int c = (int)(gid - row * G.d) * PACK_GROUP + sub * W;
+#pragma unroll
+    for (int j = 0; j < LANE_ELEMS; ++j) f[i][j] = 0.f;
+#pragma unroll
+    for (int j = 0; j < LANE_ELEMS; j += W)
+      if (gid < groups && c + j * GROUP_LANES < D) load_w<W>(x + (int64_t)row * xrs + c + j * GROUP_LANES, f[i] + j);
+  }
+#pragma unroll
+  for (int i = 0; i < ROW_ITEMS; ++i) {
+    const uint32_t gid = first + i * ROW_GROUPS, row = G.quotient(gid);
+    const int c = (int)(gid - row * G.d) * PACK_GROUP + sub * W;
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < LANE_ELEMS; ++j) m = max(m, finite_abs_bits(f[i][j]));
+#pragma unroll
+    for (int o = 1; o < GROUP_LANES; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (gid < groups) {
+      const uint32_t b = group_exponent(m);
+      if (sub == 0) e[gid] = (uint8_t)b;
+      const float inv = inv_scale(b);
+      if (b == TOP_EXPONENT) keep_finite(f[i]);
+      uint32_t w[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        w[j] = pack4(code_of(f[i][4 * j], inv), code_of(f[i][4 * j + 1], inv), code_of(f[i][4 * j + 2], inv), code_of(f[i][4 * j + 3], inv));
+#pragma unroll
+      for (int j = 0; j < LANE_ELEMS; j += W)
+        if (c + j * GROUP_LANES < D) store_codes<W>(q + (int64_t)row * D + c + j * GROUP_LANES, w, j);
+    }
   }
 }
 
-template <typename T>
+template <typename T, int W>
 __global__ void __launch_bounds__(PACK_THREADS) unpack_rows_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ e,
-                                                                   T* __restrict__ x, int64_t M, int D, int G, int vec) {
-  const int64_t gid = ((int64_t)blockIdx.x * PACK_THREADS + threadIdx.x) >> 3;
-  const int sub = threadIdx.x & 7;
-  if (gid >= M * G) return;
-  const int64_t row = gid / G;
-  const int c = (int)(gid - row * G) * PACK_GROUP + sub * 4;
-  if (c >= D) return;
-  const float s = __uint_as_float((uint32_t)e[gid] << 23);
-  const uint8_t* p = q + row * D + c;
-  T* d = x + row * D + c;
-  if (vec) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(p) ^ 0x80808080u;
-    const float f[4] = {value_of(w, 0, s), value_of(w, 1, s), value_of(w, 2, s), value_of(w, 3, s)};
-    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
-    else *reinterpret_cast<float4*>(d) = make_float4(f[0], f[1], f[2], f[3]);
-  } else {
+                                                                   T* __restrict__ x, uint32_t groups, int D, const FastDiv G) {
+  const int sub = threadIdx.x % GROUP_LANES;
+  const uint32_t first = blockIdx.x * (ROW_ITEMS * ROW_GROUPS) + threadIdx.x / GROUP_LANES;
+  uint32_t w[ROW_ITEMS][2], ex[ROW_ITEMS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) if (c + j < D) stf(d + j, value_of((uint32_t)(p[j] ^ 0x80u), 0, s));
+  for (int i = 0; i < ROW_ITEMS; ++i) {
+    const uint32_t gid = first + i * ROW_GROUPS, row = G.quotient(gid);
+    const int c = (int)(gid - row * G.d) * PACK_GROUP + sub * W;
+    w[i][0] = w[i][1] = ex[i] = 0u;
+    if (gid < groups) {
+#pragma unroll
+      for (int j = 0; j < LANE_ELEMS; j += W)
+        if (c + j * GROUP_LANES < D) load_codes<W>(q + (int64_t)row * D + c + j * GROUP_LANES, w[i], j);
+      ex[i] = e[gid];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROW_ITEMS; ++i) {
+    const uint32_t gid = first + i * ROW_GROUPS, row = G.quotient(gid);
+    const int c = (int)(gid - row * G.d) * PACK_GROUP + sub * W;
+    const float s = __uint_as_float(ex[i] << 23);
+    float f[LANE_ELEMS];
+#pragma unroll
+    for (int j = 0; j < LANE_ELEMS; ++j) f[j] = value_of(w[i][j >> 2] ^ 0x80808080u, j & 3, s);
+#pragma unroll
+    for (int j = 0; j < LANE_ELEMS; j += W)
+      if (gid < groups && c + j * GROUP_LANES < D) store_w<W>(x + (int64_t)row * D + c + j * GROUP_LANES, f + j);
   }
 }
+
+// elements an access may hold: rows begin at multiples of it on both sides (an access of values is 16 bytes at most)
+template <typename T> static int row_width(const void* x, int64_t xrs, const void* q, int D) {
+  for (int w = 8; w > 1; w >>= 1) {
+    const uintptr_t bytes = w * sizeof(T) < 16 ? w * sizeof(T) : 16;
+    if (D % w == 0 && xrs % w == 0 && reinterpret_cast<uintptr_t>(x) % bytes == 0 && reinterpret_cast<uintptr_t>(q) % w == 0) return w;
+  }
+  return 1;
+}
+// rows a launch takes: its groups are counted in 31 bits, the last block's overhang included
+static int64_t rows_a_launch(int64_t G) { return ((1LL << 31) - ROW_ITEMS * ROW_GROUPS) / G; }
 
 constexpr int64_t PACK_MAX_BLOCKS = 0x7fffffffLL;
 
@@ -239,11 +333,18 @@ static int pack_t(const void* x, int64_t xrs, void* q, void* e, int64_t M, int D
     ORBIT_CHECK_LAUNCH("pack_flat_kernel");
     return OK;
   }
-  const int vec = D % 4 == 0 && xrs % 4 == 0 && (reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T))) == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0;
-  const int64_t blocks = (M * G * 8 + PACK_THREADS - 1) / PACK_THREADS;
-  ORBIT_REQUIRE(blocks <= PACK_MAX_BLOCKS, ERR_UNSUPPORTED, "orbit_act_pack: %lld elements are too many for one call", (long long)(M * D));
-  pack_rows_kernel<T><<<(unsigned)blocks, PACK_THREADS, 0, st>>>((const T*)x, xrs, (uint8_t*)q, (uint8_t*)e, M, D, G, vec);
-  ORBIT_CHECK_LAUNCH("pack_rows_kernel");
+  const int w = row_width<T>(x, xrs, q, D);
+  const int64_t most = rows_a_launch(G);
+  for (int64_t r = 0; r < M; r += most) {
+    const uint32_t groups = (uint32_t)((M - r < most ? M - r : most) * G), blocks = (groups + ROW_ITEMS * ROW_GROUPS - 1) / (ROW_ITEMS * ROW_GROUPS);
+    const T* xr = (const T*)x + r * xrs;
+    uint8_t *qr = (uint8_t*)q + r * D, *er = (uint8_t*)e + r * G;
+    if (w == 8) pack_rows_kernel<T, 8><<<blocks, PACK_THREADS, 0, st>>>(xr, xrs, qr, er, groups, D, FastDiv(G));
+    else if (w == 4) pack_rows_kernel<T, 4><<<blocks, PACK_THREADS, 0, st>>>(xr, xrs, qr, er, groups, D, FastDiv(G));
+    else if (w == 2) pack_rows_kernel<T, 2><<<blocks, PACK_THREADS, 0, st>>>(xr, xrs, qr, er, groups, D, FastDiv(G));
+    else pack_rows_kernel<T, 1><<<blocks, PACK_THREADS, 0, st>>>(xr, xrs, qr, er, groups, D, FastDiv(G));
+    ORBIT_CHECK_LAUNCH("pack_rows_kernel");
+  }
   return OK;
 }
 
@@ -258,11 +359,18 @@ static int unpack_t(const void* q, const void* e, void* x, int64_t M, int D, cud
     ORBIT_CHECK_LAUNCH("unpack_flat_kernel");
     return OK;
   }
-  const int vec = D % 4 == 0 && (reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T))) == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0;
-  const int64_t blocks = (M * G * 8 + PACK_THREADS - 1) / PACK_THREADS;
-  ORBIT_REQUIRE(blocks <= PACK_MAX_BLOCKS, ERR_UNSUPPORTED, "orbit_act_unpack: %lld elements are too many for one call", (long long)(M * D));
-  unpack_rows_kernel<T><<<(unsigned)blocks, PACK_THREADS, 0, st>>>((const uint8_t*)q, (const uint8_t*)e, (T*)x, M, D, G, vec);
-  ORBIT_CHECK_LAUNCH("unpack_rows_kernel");
+  const int w = row_width<T>(x, D, q, D);
+  const int64_t most = rows_a_launch(G);
+  for (int64_t r = 0; r < M; r += most) {
+    const uint32_t groups = (uint32_t)((M - r < most ? M - r : most) * G), blocks = (groups + ROW_ITEMS * ROW_GROUPS - 1) / (ROW_ITEMS * ROW_GROUPS);
+    const uint8_t *qr = (const uint8_t*)q + r * D, *er = (const uint8_t*)e + r * G;
+    T* xr = (T*)x + r * D;
+    if (w == 8) unpack_rows_kernel<T, 8><<<blocks, PACK_THREADS, 0, st>>>(qr, er, xr, groups, D, FastDiv(G));
+    else if (w == 4) unpack_rows_kernel<T, 4><<<blocks, PACK_THREADS, 0, st>>>(qr, er, xr, groups, D, FastDiv(G));
+    else if (w == 2) unpack_rows_kernel<T, 2><<<blocks, PACK_THREADS, 0, st>>>(qr, er, xr, groups, D, FastDiv(G));
+    else unpack_rows_kernel<T, 1><<<blocks, PACK_THREADS, 0, st>>>(qr, er, xr, groups, D, FastDiv(G));
+    ORBIT_CHECK_LAUNCH("unpack_rows_kernel");
+  }
   return OK;
 }
 
