@@ -3,7 +3,8 @@
 // A group of LPR lanes owns a row of the state (a value channel): the row is read and written once in float4 accesses, the dot
 // product with q is a shuffle sum.  ROWS rows a group keep that many 16-byte loads a thread in flight.  S' may be S itself:
 // every element is read and written by the same thread, read first.
-// HBM-bound: 8 bytes a state element and token.
+// HBM-bound: 8 bytes a state element and token.  2048 states of 128 x 128, bfloat16 operands, from memory: 49 us (5.5 TB/s), 8192 of
+// them 174 us (6.2 TB/s, 94% of the measured copy); 2048 states of 96 x 128: 41 us (5.0 TB/s).
 #include "common.cuh"
 #include "../../include/orbit_b200.h"
 
@@ -21,8 +22,8 @@ struct LaStepArgs {
   float scale;
 };
 
-// VEC elements an access (4, or 1 where Dk or the pointers do not allow it)
-template <typename IO, int LPR, int ROWS, int VEC>
+// VEC elements an access of the state (4, or 1 where Dk or the pointers do not allow it); QK4: q and k are read in fours as well
+template <typename IO, int LPR, int ROWS, int VEC, bool QK4>
 __global__ void __launch_bounds__(LS_THREADS) la_step_kernel(const LaStepArgs a) {
   constexpr int GROUPS = LS_THREADS / LPR;
   const int sub = threadIdx.x % LPR, grp = threadIdx.x / LPR, Dk = a.Dk, Dv = a.Dv;
@@ -55,8 +56,16 @@ __global__ void __launch_bounds__(LS_THREADS) la_step_kernel(const LaStepArgs a)
     }
     const float dec = expf(a.log_decay[h]);
     float kk[VEC], qq[VEC];
+    if constexpr (QK4) {
+      const uint2 ku = *reinterpret_cast<const uint2*>(k + x), qu = *reinterpret_cast<const uint2*>(q + x);
+      unpack_bf16(ku.x, kk[0], kk[1]);
+      unpack_bf16(ku.y, kk[2], kk[3]);
+      unpack_bf16(qu.x, qq[0], qq[1]);
+      unpack_bf16(qu.y, qq[2], qq[3]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) { kk[i] = ldf(k + x + i); qq[i] = ldf(q + x + i); }
+      for (int i = 0; i < VEC; ++i) { kk[i] = ldf(k + x + i); qq[i] = ldf(q + x + i); }
+    }
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       const int e = e0 + r * GROUPS;
@@ -81,25 +90,37 @@ __global__ void __launch_bounds__(LS_THREADS) la_step_kernel(const LaStepArgs a)
   }
 }
 
-template <typename IO, int LPR, int VEC>
+template <typename IO, int LPR, int VEC, bool QK4>
 static int step_launch(const LaStepArgs& a, int64_t heads, cudaStream_t st) {
   constexpr int ROWS = 4, GROUPS = LS_THREADS / LPR;
   const int64_t grid = heads * ((a.Dv + GROUPS * ROWS - 1) / (GROUPS * ROWS));
   ORBIT_REQUIRE(grid <= 0x7fffffffLL, ERR_UNSUPPORTED, "orbit_la_step: %lld (batch, head) states are too many for one call", (long long)heads);
-  la_step_kernel<IO, LPR, ROWS, VEC><<<(unsigned)grid, LS_THREADS, 0, st>>>(a);
+  la_step_kernel<IO, LPR, ROWS, VEC, QK4><<<(unsigned)grid, LS_THREADS, 0, st>>>(a);
   ORBIT_CHECK_LAUNCH("la_step_kernel");
   return OK;
 }
 
-// lanes a row: as many as its float4s, a power of two from 8 to 32
+// Lanes a row: 8, 16 or 32, what leaves the fewest of them without a float4 in the row's last access, the larger of equals
+// (2048 states of 128 x 72: 35 us with 8 lanes, 45 with 32; of 128 x 128: 49 us with 32 lanes).
+template <typename IO, bool QK4>
+static int step_rows(const LaStepArgs& a, int64_t heads, cudaStream_t st) {
+  const int n4 = a.Dk / 4, by8 = (n4 + 7) / 8 * 8, by16 = (n4 + 15) / 16 * 16, by32 = (n4 + 31) / 32 * 32;
+  if (by32 <= by8) return step_launch<IO, 32, 4, QK4>(a, heads, st);
+  if (by16 <= by8) return step_launch<IO, 16, 4, QK4>(a, heads, st);
+  return step_launch<IO, 8, 4, QK4>(a, heads, st);
+}
 template <typename IO>
 static int step_t(const LaStepArgs& a, int64_t heads, cudaStream_t st) {
   if (a.Dk % 4 == 0 && aligned16(a.s0) && aligned16(a.s1)) {
-    if (a.Dk <= 32) return step_launch<IO, 8, 4>(a, heads, st);
-    if (a.Dk <= 64) return step_launch<IO, 16, 4>(a, heads, st);
-    return step_launch<IO, 32, 4>(a, heads, st);
+    // bfloat16 q and k in 8-byte reads where they lie so (8192 states of 128 x 128: 182 -> 174 us; wider reads of float32 ones
+    // gained nothing)
+    if constexpr (sizeof(IO) == 2) {
+      if ((a.q_bs | a.q_hs | a.k_bs | a.k_hs) % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k)) & 7) == 0)
+        return step_rows<IO, true>(a, heads, st);
+    }
+    return step_rows<IO, false>(a, heads, st);
   }
-  return step_launch<IO, 32, 1>(a, heads, st);
+  return step_launch<IO, 32, 1, false>(a, heads, st);
 }
 
 }  // namespace orbit
