@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(LG_THREADS) la_generic_kernel(const __grid_con
   float* PT = Z + (int64_t)X4 * LG_E;                  // [s][t], row TS
   float* pw = PT + T * TS;                             // a^0 .. a^T
   float* fw = pw + T + 4;                              // write factor of each token of the chunk
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, lane = tid & 31, warp = tid >> 5;
   const double ld = (double)p.log_decay[h];
   if (tid <= T) pw[tid] = tid == 0 ? 1.f : (float)exp(ld * tid);
 
@@ -61,9 +61,26 @@ __global__ void __launch_bounds__(LG_THREADS) la_generic_kernel(const __grid_con
   const int64_t head = (int64_t)b * p.H + h;
   // the state that enters the segment (joined from the segments' shares, or the carried one)
   const float* enter = local ? nullptr : J.part ? J.part + (head * p.nseg + seg) * p.S : J.z0 ? J.z0 + head * p.S : nullptr;
-  for (int i = tid; i < X4 * LG_E; i += LG_THREADS) {
-    const int e = J.xs == 1 ? i / X4 : i % LG_E, x = J.xs == 1 ? i % X4 : i / LG_E;   // the axis that lies dense goes along threads
-    Z[x * LG_E + e] = enter && x < X && e0 + e < E ? enter[x * J.xs + (e0 + e) * J.es] : 0.f;
+  // (the axis that lies dense goes along the lanes; eight reads in flight)
+  auto z_in = [&](int x, int e) { return enter && x < X && e0 + e < E ? enter[x * J.xs + (e0 + e) * J.es] : 0.f; };
+  if (J.xs == 1) {
+    for (int x = lane; x < X4; x += 32) {
+      float r[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = z_in(x, warp * 8 + i);
+      float4* d = reinterpret_cast<float4*>(Z + x * LG_E + warp * 8);
+      d[0] = make_float4(r[0], r[1], r[2], r[3]);
+      d[1] = make_float4(r[4], r[5], r[6], r[7]);
+    }
+  } else {
+    for (int x = warp; x < X4; x += 32) {
+      float r[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { r[i][0] = z_in(x + 8 * i, lane); r[i][1] = z_in(x + 8 * i, lane + 32); }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (x + 8 * i < X4) { Z[(x + 8 * i) * LG_E + lane] = r[i][0]; Z[(x + 8 * i) * LG_E + lane + 32] = r[i][1]; }
+    }
   }
 
   const IO* q = (const IO*)J.q + b * J.q_bs + h * J.q_hs;
@@ -74,15 +91,36 @@ __global__ void __launch_bounds__(LG_THREADS) la_generic_kernel(const __grid_con
   for (int ci = 0; ci < nch; ++ci) {
     const int t0 = s0 + (rev ? nch - 1 - ci : ci) * T, Tv = min(T, s1 - t0);
     __syncthreads();
-    for (int i = tid; i < T * X4; i += LG_THREADS) {
-      const int t = i / X4, x = i - t * X4;
-      const bool in = t < Tv && x < X;
-      KT[x * TS + t] = in ? ldf(k + (int64_t)(t0 + t) * J.k_ls + x) : 0.f;
-      if (!local) QT[x * TS + t] = in ? ldf(q + (int64_t)(t0 + t) * J.q_ls + x) : 0.f;
+    // a warp owns RT tokens: its lanes read along the rows, RT reads a lane and operand in flight, and store the tokens side by
+    // side (float4, eight lanes on 32 different banks)
+    constexpr int RT = T / 8;
+    for (int x = lane; x < X4; x += 32) {
+      float rk[RT], rq[RT];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int t = warp * RT + i;
+        const bool in = t < Tv && x < X;
+        rk[i] = in ? ldf(k + (int64_t)(t0 + t) * J.k_ls + x) : 0.f;
+        rq[i] = in && !local ? ldf(q + (int64_t)(t0 + t) * J.q_ls + x) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < RT; i += 4) {
+        *reinterpret_cast<float4*>(KT + x * TS + warp * RT + i) = make_float4(rk[i], rk[i + 1], rk[i + 2], rk[i + 3]);
+        if (!local) *reinterpret_cast<float4*>(QT + x * TS + warp * RT + i) = make_float4(rq[i], rq[i + 1], rq[i + 2], rq[i + 3]);
+      }
     }
-    for (int i = tid; i < T * LG_E; i += LG_THREADS) {
-      const int t = i / LG_E, e = i % LG_E;
-      Vs[i] = (t < Tv && e0 + e < E) ? ldf(v + (int64_t)(t0 + t) * J.v_ls + e) : 0.f;
+    {
+      float rv[RT][2];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int t = warp * RT + i;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) rv[i][j] = t < Tv && e0 + lane + 32 * j < E ? ldf(v + (int64_t)(t0 + t) * J.v_ls + lane + 32 * j) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) Vs[(warp * RT + i) * LG_E + lane + 32 * j] = rv[i][j];
     }
     if (tid < T) fw[tid] = tid < Tv ? J.s_state * pw[rev ? tid + 1 : Tv - 1 - tid] : 0.f;
     __syncthreads();
@@ -205,9 +243,16 @@ __global__ void __launch_bounds__(LG_THREADS) la_generic_kernel(const __grid_con
                      : (J.z1 && seg == (rev ? 0 : p.nseg - 1) ? J.z1 + head * p.S : nullptr);
   if (!out) return;
   __syncthreads();
-  for (int i = tid; i < X4 * LG_E; i += LG_THREADS) {
-    const int e = J.xs == 1 ? i / X4 : i % LG_E, x = J.xs == 1 ? i % X4 : i / LG_E;
-    if (x < X && e0 + e < E) out[x * J.xs + (e0 + e) * J.es] = Z[x * LG_E + e];
+  if (J.xs == 1) {
+    for (int x = lane; x < X; x += 32)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (e0 + warp * 8 + i < E) out[x + (e0 + warp * 8 + i) * J.es] = Z[x * LG_E + warp * 8 + i];
+  } else {
+    for (int i = tid; i < X * LG_E; i += LG_THREADS) {
+      const int e = i % LG_E, x = i / LG_E;
+      if (e0 + e < E) out[x * J.xs + (e0 + e) * J.es] = Z[i];
+    }
   }
 }
 
