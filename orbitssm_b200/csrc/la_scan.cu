@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(LG_THREADS) la_generic_kernel(const __grid_con
     // a warp owns RT tokens: its lanes read along the rows, RT reads a lane and operand in flight, and store the tokens side by
     // side (float4, eight lanes on 32 different banks)
     constexpr int RT = T / 8;
+#pragma unroll 2
     for (int x = lane; x < X4; x += 32) {
       float rk[RT], rq[RT];
 #pragma unroll
@@ -175,8 +176,10 @@ __global__ void __launch_bounds__(LG_THREADS) la_generic_kernel(const __grid_con
         for (int j = 0; j < 4; ++j) o[i][j] *= f;
       }
       __syncthreads();
+      // (only the tokens that a row of this tile sees)
+      const int sa = rev ? ty * TM : 0, sb = rev ? T : ty * TM + TM;
 #pragma unroll 4
-      for (int s = 0; s < T; ++s) {
+      for (int s = sa; s < sb; ++s) {
         const float4 w = *reinterpret_cast<const float4*>(Vs + s * LG_E + tx * 4);
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
