@@ -174,8 +174,8 @@ def load():
 
 
 _host = None
-_HOST_ENTRIES = ("orbit_la_step", "orbit_la_fwd", "orbit_la_workspace_bytes", "orbit_block_norm_fwd", "orbit_act_pack", "orbit_act_unpack",
-                 "orbit_la_bwd")
+_HOST_ENTRIES = ("orbit_la_step", "orbit_la_fwd", "orbit_la_bwd", "orbit_la_workspace_bytes", "orbit_block_norm_fwd", "orbit_block_norm_bwd",
+                 "orbit_block_norm_bwd_workspace_bytes", "orbit_act_pack", "orbit_act_unpack")
 
 
 def host():

@@ -177,9 +177,14 @@ class BlockNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, h, gate, scale, w_post, w_pre, eps):
-        r, n, saved = _block_norm(x, h, gate, scale, w_post, w_pre, eps, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*saved)
+        got = native("block_norm", x, h, gate, scale, w_post, w_pre, eps, True)
+        if got is not None:
+            r, n, rh, rr = got
+            ctx.save_for_backward(x, h, gate, scale, w_post, w_pre, rh, rr)
+        else:
+            r, n, saved = _block_norm(x, h, gate, scale, w_post, w_pre, eps, True)
+            ctx.save_for_backward(*saved)
         ctx.meta = (x.shape, [None if t is None else t.dtype for t in (scale, w_post, w_pre)])
         return r, n
 
@@ -188,13 +193,17 @@ class BlockNormFn(torch.autograd.Function):
     def backward(ctx, dr, dn):
         if dr is None and dn is None:
             return (None,) * 7
-        x2, h2, g2, s32, wo, wi, rh, rr = ctx.saved_tensors
+        x, h, gate, s32, wo, wi, rh, rr = ctx.saved_tensors
         shape, dts = ctx.meta
-        D = shape[-1]
-        dr2 = None if dr is None else dr.contiguous().view(-1, D)
-        dn2 = None if dn is None else dn.contiguous().view(-1, D)
         need = ctx.needs_input_grad
-        dx, dh, dg, *sums = block_norm_bwd(x2, h2, g2, s32, wo, wi, rh, rr, dr2, dn2, want_sums=any(need[3:6]))
+        want_sums = need[3] or need[4] or need[5]
+        got = native("block_norm_bwd", x, h, gate, s32, wo, wi, rh, rr, dr, dn, want_sums)
+        if got is None:
+            D = shape[-1]
+            x2, h2, g2, dr2, dn2 = (None if t is None else _rows_of(t, D) for t in (x, h, gate, dr, dn))
+            dr2, dn2 = (None if t is None else t.contiguous() for t in (dr2, dn2))
+            got = block_norm_bwd(x2, h2, g2, s32, wo, wi, rh, rr, dr2, dn2, want_sums=want_sums)
+        dx, dh, dg, *sums = got
         out = [dx.view(shape) if need[0] else None, dh.view(shape) if need[1] else None,
                dg.view(shape) if need[2] else None]
         out += [s.to(dt) if (need[3 + i] and s is not None) else None for i, (s, dt) in enumerate(zip(sums, dts))]
@@ -211,7 +220,7 @@ def block_norm(x, h, *, gate=None, scale=None, post_weight=None, pre_weight=None
     x, h, gate: [..., D] of one shape and dtype (float32 or bfloat16; a column slice of a wider buffer is read in place);
     scale, post_weight, pre_weight: [D].  Returns (r, n) in the dtype of x; arithmetic, norms and the weights' gradients are
     float32, and n is formed from the unrounded r.  First-order differentiable in every tensor argument."""
-    got = native("block_norm", x, h, gate, scale, post_weight, pre_weight, eps)
+    got = native("block_norm", x, h, gate, scale, post_weight, pre_weight, eps, False)
     if got is not None:
         return tuple(got)
     who = "block_norm"

@@ -1,7 +1,8 @@
-// Host side of the block operators' calls that record no gradient: checks, output tensors and the launch in one native call.
+// Host side of the block operators' calls: checks, output tensors and the launch in one native call.
 //
 // A call of these operators on small inputs (one token, one decode batch) costs the host several times what it costs the GPU;
-// checks and ctypes in Python are most of it (measured on the B200 host, us a call: step 16, block norm 17, pack 12, unpack 9).
+// checks and ctypes in Python are most of it (measured on the B200 host, us a call: step 16 -> 8, block norm 17 -> 8, an activation
+// to eight bits and back 21 -> 11; a block norm with its backward pass 200 -> 170, the rest of it autograd's own).
 // Each function here serves the ordinary call and returns None for every other one (a CPU tensor, mixed dtypes, a gradient to
 // record, operands that would have to be copied, ...); the Python operator then takes its own way, which serves the call or refuses
 // it by name.  The kernels and the C-ABI entry points are the same on both ways; this file holds no arithmetic.
@@ -14,6 +15,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <cstring>
+#include <initializer_list>
 
 #include "../../include/orbit_b200.h"
 
@@ -26,6 +29,8 @@ struct Entry {
   decltype(&orbit_la_bwd) la_bwd;
   decltype(&orbit_la_workspace_bytes) la_workspace;
   decltype(&orbit_block_norm_fwd) block_norm;
+  decltype(&orbit_block_norm_bwd) block_norm_bwd;
+  decltype(&orbit_block_norm_bwd_workspace_bytes) block_workspace;
   decltype(&orbit_act_pack) pack;
   decltype(&orbit_act_unpack) unpack;
 } entry = {};
@@ -56,18 +61,19 @@ bool f32_vector(const at::Tensor& t, int64_t n) {
 constexpr int MAX_DEVICES = 64;
 int* status_word[MAX_DEVICES] = {};
 
-// (outputs..., status, launches): the caller raises for a nonzero status
-PyObject* result(int status, const at::Tensor& a, const at::Tensor& b, int launches = 1) {
-  PyObject* x = THPVariable_Wrap(a);
-  PyObject* y = b.defined() ? THPVariable_Wrap(b) : Py_NewRef(Py_None);
-  PyObject* s = PyLong_FromLong(status);
-  PyObject* l = PyLong_FromLong(launches);
-  PyObject* out = (x && y && s && l) ? PyTuple_Pack(4, x, y, s, l) : nullptr;
-  Py_XDECREF(x);
-  Py_XDECREF(y);
-  Py_XDECREF(s);
-  Py_XDECREF(l);
-  return out;
+// (outputs..., status, launches), None for an output that is not there: the caller raises for a nonzero status
+PyObject* result(int status, std::initializer_list<at::Tensor> outs, int launches = 1) {
+  PyObject* t = PyTuple_New((Py_ssize_t)outs.size() + 2);
+  if (t == nullptr) return nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor& x : outs) PyTuple_SET_ITEM(t, i++, x.defined() ? THPVariable_Wrap(x) : Py_NewRef(Py_None));
+  PyTuple_SET_ITEM(t, i++, PyLong_FromLong(status));
+  PyTuple_SET_ITEM(t, i, PyLong_FromLong(launches));
+  if (PyErr_Occurred()) {
+    Py_DECREF(t);
+    return nullptr;
+  }
+  return t;
 }
 
 #define GUARDED(...)                                         \
@@ -118,7 +124,7 @@ PyObject* la_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int rc = entry.la_step(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
                                  v.stride(1), ptr<float>(ld), ptr<float>(s), ptr<float>(s1), y.data_ptr(), (int)B, (int)H, (int)Dk, (int)Dv,
                                  (float)scale, code, stream(dev));
-    return result(rc, y, s1);
+    return result(rc, {y, s1});
   })
 }
 
@@ -163,7 +169,7 @@ PyObject* la_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.workspace = ws.data_ptr();
     }
     const int rc = entry.la_fwd(&p, code, stream(dev));
-    return result(rc, y, s1, p.workspace_bytes ? 3 : 1);
+    return result(rc, {y, s1}, p.workspace_bytes ? 3 : 1);
   })
 }
 
@@ -211,37 +217,77 @@ PyObject* la_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.workspace = ws.data_ptr();
     }
     const int rc = entry.la_bwd(&p, code, stream(dev));
-    PyObject* o[6] = {THPVariable_Wrap(dq), THPVariable_Wrap(dk), THPVariable_Wrap(dv), ds0.defined() ? THPVariable_Wrap(ds0) : Py_NewRef(Py_None),
-                      PyLong_FromLong(rc), PyLong_FromLong(p.workspace_bytes ? 3 : 1)};
-    PyObject* out = o[0] && o[1] && o[2] && o[3] && o[4] && o[5] ? PyTuple_Pack(6, o[0], o[1], o[2], o[3], o[4], o[5]) : nullptr;
-    for (PyObject* x : o) Py_XDECREF(x);
-    return out;
+    return result(rc, {dq, dk, dv, ds0}, p.workspace_bytes ? 3 : 1);
   })
 }
 
-// block_norm(x, h, gate | None, scale | None, post | None, pre | None, eps) of dense operands
-PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 7) Py_RETURN_NONE;
-  GUARDED({
-    const int dev = device_for(a[0]);
-    if (dev < 0) Py_RETURN_NONE;
-    at::Tensor x, h, g, sc, post, pre;
-    if (!plain(a[0], x, dev) || !plain(a[1], h, dev) || !plain_or_none(a[2], g, dev) || !plain_or_none(a[3], sc, dev) ||
+// The operands of a block norm: activations of one dense shape, float32 weights of its width; false for the other way.
+struct BlockOperands {
+  at::Tensor x, h, g, sc, post, pre;
+  int dev, code;
+  int64_t M, D;
+  bool take(PyObject* const* a) {
+    dev = device_for(a[0]);
+    if (dev < 0 || !plain(a[0], x, dev) || !plain(a[1], h, dev) || !plain_or_none(a[2], g, dev) || !plain_or_none(a[3], sc, dev) ||
         !plain_or_none(a[4], post, dev) || !plain_or_none(a[5], pre, dev))
-      Py_RETURN_NONE;
-    const int code = io_code(x);
+      return false;
+    code = io_code(x);
+    if (code < 0 || x.dim() < 1 || x.numel() == 0 || x.size(-1) > (1 << 30) || !x.is_contiguous() || !like_x(h) || (g.defined() && !like_x(g))) return false;
+    D = x.size(-1);
+    M = x.numel() / D;
+    return f32_vector(sc, D) && f32_vector(post, D) && f32_vector(pre, D);
+  }
+  bool like_x(const at::Tensor& t) const { return t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.is_contiguous(); }
+  at::Tensor floats(int64_t n) const { return at::empty({n}, x.options().dtype(at::kFloat)); }
+};
+
+// block_norm(x, h, gate | None, scale | None, post | None, pre | None, eps, keep) -> (r, n | None[, rstd_h | None, rstd_r | None])
+PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 8) Py_RETURN_NONE;
+  GUARDED({
+    BlockOperands o;
+    if (!o.take(a)) Py_RETURN_NONE;
     const double eps = PyFloat_AsDouble(a[6]);
     if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
-    if (code < 0 || x.dim() < 1 || x.numel() == 0 || x.size(-1) > (1 << 30) || !x.is_contiguous() || h.sizes() != x.sizes() || h.scalar_type() != x.scalar_type() ||
-        !h.is_contiguous() || (g.defined() && (g.sizes() != x.sizes() || g.scalar_type() != x.scalar_type() || !g.is_contiguous())) || !(eps >= 0.))
+    if (!(eps >= 0.)) Py_RETURN_NONE;
+    const bool keep = PyObject_IsTrue(a[7]) == 1;
+    at::Tensor r = at::empty_like(o.x), y, rh, rr;
+    if (o.pre.defined()) y = at::empty_like(o.x);
+    if (keep && o.post.defined()) rh = o.floats(o.M);
+    if (keep && o.pre.defined()) rr = o.floats(o.M);
+    const int rc = entry.block_norm(o.x.data_ptr(), o.D, o.h.data_ptr(), o.D, ptr<void>(o.g), o.D, ptr<float>(o.sc), ptr<float>(o.post),
+                                    ptr<float>(o.pre), r.data_ptr(), ptr<void>(y), ptr<float>(rh), ptr<float>(rr), o.M, (int)o.D, (float)eps,
+                                    o.code, stream(o.dev));
+    return keep ? result(rc, {r, y, rh, rr}) : result(rc, {r, y});
+  })
+}
+
+// block_norm_bwd(x, h, gate | None, scale | None, post | None, pre | None, rstd_h | None, rstd_r | None, dr | None, dn | None, want sums)
+// -> (dx, dh, dgate | None, dscale | None, dpost | None, dpre | None); the first eight are what the forward pass kept
+PyObject* block_norm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 11) Py_RETURN_NONE;
+  GUARDED({
+    BlockOperands o;
+    at::Tensor rh, rr, dr, dn;
+    if (!o.take(a) || !plain_or_none(a[6], rh, o.dev) || !plain_or_none(a[7], rr, o.dev) || !plain_or_none(a[8], dr, o.dev) ||
+        !plain_or_none(a[9], dn, o.dev))
       Py_RETURN_NONE;
-    const int64_t D = x.size(-1), M = x.numel() / D;
-    if (!f32_vector(sc, D) || !f32_vector(post, D) || !f32_vector(pre, D)) Py_RETURN_NONE;
-    at::Tensor r = at::empty_like(x), y;
-    if (pre.defined()) y = at::empty_like(x);
-    const int rc = entry.block_norm(x.data_ptr(), D, h.data_ptr(), D, ptr<void>(g), D, ptr<float>(sc), ptr<float>(post), ptr<float>(pre),
-                                    r.data_ptr(), ptr<void>(y), nullptr, nullptr, M, (int)D, (float)eps, code, stream(dev));
-    return result(rc, r, y);
+    if ((dr.defined() && !o.like_x(dr)) || (dn.defined() && !o.like_x(dn)) || o.post.defined() != rh.defined() || o.pre.defined() != rr.defined() ||
+        !f32_vector(rh, o.M) || !f32_vector(rr, o.M))
+      Py_RETURN_NONE;
+    const bool sums = PyObject_IsTrue(a[10]) == 1;
+    at::Tensor dx = at::empty_like(o.x), dh = at::empty_like(o.x), dg, ds, dpost, dpre, ws;
+    if (o.g.defined()) dg = at::empty_like(o.x);
+    if (sums && o.sc.defined()) ds = o.floats(o.D);
+    if (sums && o.post.defined()) dpost = o.floats(o.D);
+    if (sums && o.pre.defined()) dpre = o.floats(o.D);
+    const int64_t bytes = ds.defined() || dpost.defined() || dpre.defined() ? entry.block_workspace(o.M, (int)o.D) : 0;
+    if (bytes) ws = at::empty({bytes}, o.x.options().dtype(at::kByte));
+    const int rc = entry.block_norm_bwd(o.x.data_ptr(), o.D, o.h.data_ptr(), o.D, ptr<void>(o.g), o.D, ptr<float>(o.sc), ptr<float>(o.post),
+                                        ptr<float>(o.pre), ptr<float>(rh), ptr<float>(rr), ptr<void>(dr), ptr<void>(dn), dx.data_ptr(),
+                                        dh.data_ptr(), ptr<void>(dg), ptr<float>(ds), ptr<float>(dpost), ptr<float>(dpre), ptr<void>(ws), bytes,
+                                        o.M, (int)o.D, o.code, stream(o.dev));
+    return result(rc, {dx, dh, dg, ds, dpost, dpre}, bytes ? 2 : 1);
   })
 }
 
@@ -261,7 +307,7 @@ PyObject* pack(PyObject*, PyObject* const* a, Py_ssize_t n) {
     shape.back() = (D + 31) / 32;
     at::Tensor e = at::empty(shape, x.options().dtype(at::kByte));
     const int rc = entry.pack(x.data_ptr(), D, q.data_ptr(), e.data_ptr(), M, (int)D, code, stream(dev));
-    return result(rc, q, e);
+    return result(rc, {q, e});
   })
 }
 
@@ -281,26 +327,22 @@ PyObject* unpack(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t D = q.size(-1);
     at::Tensor x = at::empty(q.sizes(), q.options().dtype(half ? at::kBFloat16 : at::kFloat));
     const int rc = entry.unpack(q.data_ptr(), e.data_ptr(), x.data_ptr(), q.numel() / D, (int)D, half ? ORBIT_BF16 : ORBIT_F32, stream(dev));
-    return result(rc, x, at::Tensor());
+    return result(rc, {x});
   })
 }
 
 // bind(addresses of the entry points, in the order of `Entry`)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* p[7];
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "bind takes seven addresses");
+  constexpr int N = 9;
+  static_assert(sizeof(Entry) == N * sizeof(void*), "one address an entry");
+  void* p[N];
+  if (n != N) {
+    PyErr_Format(PyExc_TypeError, "bind takes %d addresses", N);
     return nullptr;
   }
-  for (int i = 0; i < 7; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
+  for (int i = 0; i < N; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
   if (PyErr_Occurred()) return nullptr;
-  entry.la_step = reinterpret_cast<decltype(entry.la_step)>(p[0]);
-  entry.la_fwd = reinterpret_cast<decltype(entry.la_fwd)>(p[1]);
-  entry.la_workspace = reinterpret_cast<decltype(entry.la_workspace)>(p[2]);
-  entry.block_norm = reinterpret_cast<decltype(entry.block_norm)>(p[3]);
-  entry.pack = reinterpret_cast<decltype(entry.pack)>(p[4]);
-  entry.unpack = reinterpret_cast<decltype(entry.unpack)>(p[5]);
-  entry.la_bwd = reinterpret_cast<decltype(entry.la_bwd)>(p[6]);
+  std::memcpy(&entry, p, sizeof(entry));
   Py_RETURN_NONE;
 }
 
@@ -320,7 +362,7 @@ PyObject* bind_status(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD("bind", bind),     METHOD("la_step", la_step), METHOD("la_fwd", la_fwd), METHOD("block_norm", block_norm),
                          METHOD("pack", pack),     METHOD("unpack", unpack),
-                         METHOD("bind_status", bind_status), METHOD("la_bwd", la_bwd), {nullptr, nullptr, 0, nullptr}};
+                         METHOD("bind_status", bind_status), METHOD("la_bwd", la_bwd), METHOD("block_norm_bwd", block_norm_bwd), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_orbit_host", "Native host calls of the block operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -3,6 +3,8 @@
 Tolerances are elementwise majorants, derived before the first run.  With u the half step of a type relative to the value
 (2^-8 bfloat16, 2^-24 float32) and |.|-sums M taken over absolute values, a result that is a float32 sum of n terms is off by
 at most n u32 M; an operand rounded to bfloat16 adds u16 M of its own sum, and the rounding of the result u |result|."""
+import itertools
+
 import pytest
 import torch
 
@@ -217,6 +219,41 @@ def test_a_split_sequence_equals_the_whole(dtype):
     big = majorant(q, k, v, ld, s0, 128 ** -0.5)
     close(torch.cat([a, b], 1), y.double(), 2 * big[0], dtype, 600, U16 if dtype == BF else 0.0)
     close(s, s1.double(), 2 * big[1], F32, 600, 0.0)
+
+
+# many heads (a CTA walks a whole head), few heads and long sequences (segments, joined), both; odd lengths, narrow and wide heads
+SPREADS = [(5, 300, 40, 128, 96), (4, 130, 37, 64, 128), (1, 2001, 2, 128, 128), (2, 1300, 9, 40, 128), (1, 4099, 1, 128, 64),
+           (2, 1025, 37, 128, 128)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("case", SPREADS)
+def test_attention_spread_over_the_gpu_in_other_ways(case, dtype):
+    q, k, v, ld, s0, dy, ds1 = _inputs(*case, dtype, 51)
+    _check_all(q, k, v, ld, s0, dy, ds1, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("decay", ["none", "strong", "all"])
+def test_joined_segments_at_the_ends_of_the_decay_range(decay, dtype):
+    q, k, v, ld, s0, dy, ds1 = _inputs(1, 1999, 2, 128, 72, dtype, 52, decay)
+    before = ops.LAUNCHES
+    ob.linear_attention(q, k, v, ld, s0)
+    assert ops.LAUNCHES - before == 3                                              # it is split: shares, join, walk
+    _check_all(q, k, v, ld, s0, dy, ds1, dtype)
+
+
+def test_one_token_is_the_step():
+    for dtype in (BF, F32):
+        q, k, v, ld, s0, _, _ = _inputs(3, 1, 4, 72, 128, dtype, 53)
+        y, s1 = ob.linear_attention(q, k, v, ld, s0, return_state=True)
+        z, s2 = ob.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s0)
+        big = majorant(q, k, v, ld, s0, 72 ** -0.5)
+        close(y[:, 0], z.double(), 2 * big[0][:, 0], dtype, 300, U16 if dtype == BF else 0.0)
+        close(s1, s2.double(), 2 * big[1], F32, 300, 0.0)
+        wide = torch.cat([v, v], 3)[..., :128]                                     # strided rows of one token
+        a, b = ob.linear_attention(q, k, wide, ld, s0, return_state=True)
+        assert torch.equal(a, y) and torch.equal(b, s1)
 
 
 def test_rows_of_other_sequences_do_not_matter_and_repeats_are_bitwise():
@@ -476,6 +513,37 @@ def test_native_host_calls_and_the_python_way_give_the_same_bits():
         finally:
             ops.set_timing(None)
         assert len(native) == len(python) and all(torch.equal(a, b) for a, b in zip(native, python))
+
+
+@pytest.mark.parametrize("dtype", (BF, F32))
+def test_block_norm_gradients_on_either_host_way_are_the_same_bits(dtype):
+    g = _gen(43)
+    x, h, z, dr, dn = (_randn(g, 3, 11, 72, dtype=dtype) for _ in range(5))
+    s, wo, wi = (_randn(g, 72) for _ in range(3))
+
+    def run(gate, post, scale, need):
+        ins = [t.clone().requires_grad_(i in need) for i, t in enumerate((x, h, z, s, wo, wi))]
+        a = [ins[0], ins[1], ins[2] if gate else None, ins[3] if scale else None, ins[4] if post else None, ins[5]]
+        r, n = ob.block_norm(a[0], a[1], gate=a[2], scale=a[3], post_weight=a[4], pre_weight=a[5])
+        leaves = [t for t in a if t is not None and t.requires_grad]
+        out = [r, n, *torch.autograd.grad((r, n), leaves, (dr, dn), retain_graph=True)]
+        out += torch.autograd.grad(n, leaves, dn, retain_graph=True, allow_unused=True)
+        return out + list(torch.autograd.grad(r, leaves, dr[:, :1].expand_as(r), allow_unused=True))
+
+    for gate, post, scale in itertools.product((True, False), repeat=3):
+        for need in ((0, 1, 2, 3, 4, 5), (0, 1, 2), (3, 4, 5), (1,)):
+            before = ops.LAUNCHES
+            native = run(gate, post, scale, need)
+            launches = ops.LAUNCHES - before
+            ops.set_timing([])                            # a timed region takes the Python way
+            try:
+                before = ops.LAUNCHES
+                python = run(gate, post, scale, need)
+                assert ops.LAUNCHES - before == launches
+            finally:
+                ops.set_timing(None)
+            for a, b in zip(native, python, strict=True):
+                assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
 
 
 def test_calls_on_tensors_of_another_type_or_place_are_refused_on_the_gpu_too():
