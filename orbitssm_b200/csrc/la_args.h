@@ -40,7 +40,7 @@ int la_plan(const LaArgs& a, bool bwd, int nseg, int seg_len, bool local, LaPlan
 // the launch between the two: shares of the segments -> states that enter them, in place, for the jobs of the state-only plan
 int la_join(const LaPlan& p, cudaStream_t st);
 // segments the sequence is split into so that `units` CTAs per segment fill the GPU (chunk = tokens of one tile)
-int la_segments(int64_t units, int L, int chunk, int* seg_len, double* cost = nullptr);
+int la_segments(int64_t units, int L, int chunk, double setup, double join, int* seg_len, double* cost = nullptr);
 
 bool la_tc_serves(const LaArgs& a, bool bwd, int dtype);
 int la_tc_launch(const LaArgs& a, bool bwd, cudaStream_t st);

@@ -14,7 +14,9 @@
 // its segment from there.  No CTA waits on another.
 //
 // One CTA of 256 threads owns a head's segment and 64 output channels; 4 x 4 register tiles (float4 reads of operands that
-// are kept transposed in shared memory).  Bound by the FP32 pipe and shared-memory reads.
+// are kept transposed in shared memory).  The FP32 pipe bounds it: a chunk of 64 tokens of a 128 x 64 tile is 14000 cycles of FMAs,
+// and the chunks take 1.9 times that (half of the scores are masked work, and the reads of a chunk are not hidden).  Measured in
+// float32: [8, 4096, 16, 128, 128] 2771 us, [2, 777, 8, 64, 64] forward 53 us and backward 99.
 #include "common.cuh"
 #include "la_args.h"
 #include <math.h>
@@ -345,10 +347,12 @@ int la_plan(const LaArgs& a, bool bwd, int nseg, int seg_len, bool local, LaPlan
   return OK;
 }
 
-// The split that takes the fewest chunk steps on 148 SMs: rounds of CTAs times the chunks of a segment and three steps' worth of
-// set-up; for more than one segment also the first launch, which reads half of the operands and costs about half a step for each,
-// and the join, about two steps.  At most 32 segments: more would only fill rounds that are full.
-int la_segments(int64_t units, int L, int chunk, int* seg_len, double* cost_out) {
+// The split that takes the fewest chunk steps on 148 SMs: rounds of CTAs times the chunks of a segment and `setup` steps' worth of
+// prologue and state; for more than one segment also the first launch, which reads half of the operands and costs about half a step
+// for each, and `join` steps for the launch between the two.  At most 32 segments: more would only fill rounds that are full.
+// (Tensor-core tiles, 16 heads of 128 x 128, one segment against the split taken: 2048 tokens 51 us and 47, 8192 tokens 167 and 87,
+// 65536 tokens 1233 and 341.  Float32, [2, 777, 8, 64, 64]: 156 and 53.)
+int la_segments(int64_t units, int L, int chunk, double setup, double join, int* seg_len, double* cost_out) {
   const int nch = (L + chunk - 1) / chunk;
   int best = 1, best_len = nch;
   double best_cost = 0.;
@@ -356,7 +360,7 @@ int la_segments(int64_t units, int L, int chunk, int* seg_len, double* cost_out)
     const int per = (nch + n - 1) / n, ns = (nch + per - 1) / per;
     if (ns != n) continue;
     const int64_t rounds = (units * n + 147) / 148, first = (units * (n - 1) + 147) / 148;
-    const double cost = (double)rounds * (per + 3) + (n > 1 ? 0.5 * (double)first * (per + 3) + 2. : 0.);
+    const double cost = (double)rounds * (per + setup) + (n > 1 ? 0.5 * (double)first * (per + setup) + join : 0.);
     if (n == 1 || cost < 0.95 * best_cost) { best = n; best_len = per; best_cost = cost; }
   }
   *seg_len = best_len * chunk;
@@ -367,7 +371,7 @@ int la_segments(int64_t units, int L, int chunk, int* seg_len, double* cost_out)
 static int lg_chunk(const LaArgs& a) { return a.Dk <= 128 && a.Dv <= 128 ? 64 : 32; }
 static int lg_segments(const LaArgs& a, bool bwd, int* seg_len) {
   const int64_t ev = (a.Dv + LG_E - 1) / LG_E, ek = (a.Dk + LG_E - 1) / LG_E;
-  return la_segments((int64_t)a.B * a.H * (bwd ? 2 * ek + ev : ev), a.L, lg_chunk(a), seg_len);
+  return la_segments((int64_t)a.B * a.H * (bwd ? 2 * ek + ev : ev), a.L, lg_chunk(a), 1., 1., seg_len);
 }
 
 template <typename IO, int T>
@@ -439,8 +443,8 @@ extern "C" int orbit_la_fwd(const orbit_la_args* a, int dtype, void* stream) {
     return OK;
   }
   ORBIT_REQUIRE(a->q && a->k && a->v && a->y && a->log_decay, ERR_BAD_ARG, "orbit_la_fwd: null q/k/v/y/log_decay");
-  // One token with a state on either side is the decode step: its kernel takes a third of the time of a tile with one row (at 16
-  // heads of 128 x 128: 5 us against 14).
+  // One token with a state on either side is the decode step (16 heads of 128 x 128: 9 us a call against 14 of a tile with one
+  // row).
   if (a->L == 1 && a->state0 && a->state1 && (a->H == 1 || a->y_hs == a->Dv) && (a->B == 1 || a->y_bs == (int64_t)a->H * a->Dv))
     return orbit_la_step(a->q, a->q_bs, a->q_hs, a->k, a->k_bs, a->k_hs, a->v, a->v_bs, a->v_hs, a->log_decay, a->state0, a->state1, a->y,
                          a->B, a->H, a->Dk, a->Dv, a->scale, dtype, stream);

@@ -18,7 +18,11 @@
 //
 // What bounds it is shared-memory bandwidth (the MMAs' operands) and the power limit, so operands are kept out of shared memory
 // where TMEM can hold them: per chunk and head of 128 x 128 the tiles move 96 KB in, 288 KB to the MMAs and 160 KB for the element
-// passes.  (With the parts of f v' in shared memory and 64 channels a CTA it was 800 KB and twice the time.)
+// passes.  (With the parts of f v' in shared memory and 64 channels a CTA it was 800 KB, and 158 us where it now takes 119.)
+// Measured: forward [8, 4096, 16, 128, 128] 114 to 119 us (4.5 to 4.7 TB/s of operands and output), backward 360 us; prompt
+// [1, 65536, 16, 128, 128] 341 us.  Random operands draw 1000 W and the SM clock falls to 1.4 to 1.6 GHz; zeros run 20% faster.
+// bfloat16 calls that these tiles do not serve take the float32 kernels, which need 80 us for [1, 131, 16, 128, 128] where these
+// need 17, and 3827 us for [8, 4096, 16, 128, 128].
 //
 // Warp-specialised, 28 warps that meet only through mbarriers (every wait bounded):
 //   warps 0..3   decay mask: S1 -> P, in the place of S1 (thread = row t)
@@ -637,16 +641,18 @@ bool la_tc_serves(const LaArgs& a, bool bwd, int dtype) {
 
 // How a call is spread over the SMs: segments of the sequence, and for heads wider than 64 channels one CTA a head or one for each
 // half of its channels (`ne`).  A half costs three quarters of a whole chunk step (scores and the products of the state are made for
-// either half), but needs no first launch; so it is taken where it fills SMs that segments would fill at a higher price.
+// either half), but needs no first launch; so it is taken where it fills SMs that segments would fill at a higher price.  Heads of
+// 128 x 128, whole heads against halves: [1, 131, 16] 20 us and 16, [1, 2048, 16] 53 and 47; [8, 4096, 16] 113 and 183, [1, 65536, 16]
+// 341 and 594.  Prologue and state cost about three steps a CTA, the joining launch five (with two: [2, 1000, 8] 38 us instead of 31).
 static int tc_split(const LaArgs& a, bool bwd, int* seg_len, int* ne) {
   const int64_t heads = (int64_t)a.B * a.H;
   const int wide = (a.Dv > 64) + (bwd ? 2 * (a.Dk > 64) : 0), jobs = bwd ? 3 : 1;
   double whole = 0., halves = 0.;
-  const int n1 = la_segments(heads * jobs, a.L, LT_T, seg_len, &whole);
+  const int n1 = la_segments(heads * jobs, a.L, LT_T, 3., 5., seg_len, &whole);
   *ne = 1;
   if (wide == 0) return n1;
   int len2 = 0;
-  const int n2 = la_segments(heads * (jobs + wide), a.L, LT_T, &len2, &halves);
+  const int n2 = la_segments(heads * (jobs + wide), a.L, LT_T, 3., 5., &len2, &halves);
   if (0.75 * halves >= 0.95 * whole) return n1;
   *ne = 2;
   *seg_len = len2;
