@@ -135,8 +135,14 @@ class LinearAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, scale, want_state, slots):
-        y, new, saved = _la(q, k, v, log_decay, state, scale, want_state)
         ctx.set_materialize_grads(False)
+        got = native("la_fwd", q, k, v, log_decay, state, scale, want_state)     # (checks the call as well)
+        if got is not None:
+            y, new = got
+            saved = (q, k, v, log_decay, state)
+        else:
+            scale, log_decay = _checked(q, k, v, log_decay, state, scale)
+            y, new, saved = _la(q, k, v, log_decay, state, scale, want_state)
         ctx.save_for_backward(*saved)
         ctx.scale, ctx.slots = scale, slots
         return y, new
@@ -158,7 +164,8 @@ class LinearAttentionFn(torch.autograd.Function):
                     view = slot[0].view(slot[1], dy.new_empty((1,)).expand(B, L, H * D))     # a tensor of the range's shape
                     if view is not None and _operand(view.unflatten(2, (H, D))).data_ptr() == view.data_ptr():
                         outs[i] = view.unflatten(2, (H, D))
-        dq, dk, dv, ds0 = la_bwd(q, k, v, log_decay, s0, ctx.scale, dy, dstate, need[4] and s0 is not None, outs)
+        scale = ctx.scale if ctx.scale is not None else q.shape[-1] ** -0.5
+        dq, dk, dv, ds0 = la_bwd(q, k, v, log_decay, s0, scale, dy, dstate, need[4] and s0 is not None, outs)
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, ds0 if need[4] else None,
                 None, None, None)
 
@@ -195,6 +202,13 @@ def _scale_of(who, scale, Dk):
     return scale
 
 
+def _checked(q, k, v, log_decay, state, scale):
+    """Refuses what `linear_attention` does not serve -> the scale and the decays as the kernels take them."""
+    _check_operands("linear_attention", q, k, v, log_decay, state, ("B", "L"))
+    scale = _scale_of("linear_attention", scale, q.shape[-1])
+    return scale, log_decay if log_decay.is_contiguous() and not log_decay.requires_grad else log_decay.detach().contiguous()
+
+
 def linear_attention(q, k, v, log_decay, state=None, *, scale=None, return_state=False, _slots=None):
     """y_t = scale S_t q_t over a sequence, with S_t = exp(log_decay) S_{t-1} + v_t k_t^T for each head.
 
@@ -206,19 +220,16 @@ def linear_attention(q, k, v, log_decay, state=None, *, scale=None, return_state
     bfloat16 heads whose widths are multiples of 8 up to 128 run on tensor-core tiles: products of the unrounded inputs with the
     scores or the state rounded once to bfloat16, float32 sums; the state itself is float32 throughout.  Other calls run on
     float32 kernels.  Values are expected to be finite: a NaN or infinity may reach every output of its head and sequence."""
-    got = native("la_fwd", q, k, v, log_decay, state, scale, return_state)
-    if got is not None:
-        return tuple(got) if return_state else got[0]
-    who = "linear_attention"
-    _check_operands(who, q, k, v, log_decay, state, ("B", "L"))
-    scale, return_state = _scale_of(who, scale, q.shape[-1]), bool(return_state)
-    if not log_decay.is_contiguous() or log_decay.requires_grad:
-        log_decay = log_decay.detach().contiguous()
+    if log_decay.requires_grad:
+        _checked(q, k, v, log_decay, state, scale)               # refuses a gradient of it
     if wants_grad(q, k, v, state):
-        y, new = LinearAttentionFn.apply(q, k, v, log_decay, state, scale, return_state, _slots)
-    else:
-        y, new, _ = _la(q, k, v, log_decay, state, scale, return_state)
-    return (y, new) if return_state else y
+        y, new = LinearAttentionFn.apply(q, k, v, log_decay, state, scale, bool(return_state), _slots)
+        return (y, new) if return_state else y
+    got = native("la_fwd", q, k, v, log_decay, state, scale, return_state)
+    if got is None:
+        scale, log_decay = _checked(q, k, v, log_decay, state, scale)
+        got = _la(q, k, v, log_decay, state, scale, bool(return_state))
+    return (got[0], got[1]) if return_state else got[0]
 
 
 def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out_state=None):
