@@ -261,23 +261,33 @@ __global__ void __launch_bounds__(LG_THREADS) la_generic_kernel(const __grid_con
   }
 }
 
-// One thread an element of a head's state: walks the segments in the direction's order, in place.
+// One thread an element of a head's state: walks the segments in the direction's order, in place, eight reads in flight.
 __global__ void __launch_bounds__(256) la_join_kernel(const __grid_constant__ LaPlan p) {
+  constexpr int AHEAD = 8;
   const LaJob& J = p.job[blockIdx.y];
   const int blocks = (p.S + 255) / 256, rev = J.reverse, n = p.nseg;
   const int i = (int)(blockIdx.x % blocks) * 256 + threadIdx.x;
   const int64_t head = blockIdx.x / blocks;
   if (i >= p.S) return;
-  const double ld = (double)p.log_decay[head % p.H];
-  const float full = (float)exp(ld * p.seg_len), last = (float)exp(ld * (p.L - (n - 1) * p.seg_len));
   float* part = J.part + head * n * p.S + i;
   float z = J.z0 ? J.z0[head * p.S + i] : 0.f;
-#pragma unroll 4
-  for (int k = 0; k < n; ++k) {
-    const int s = rev ? n - 1 - k : k;
-    const float share = k < n - 1 ? part[(int64_t)s * p.S] : 0.f;          // nobody formed the last one's
-    part[(int64_t)s * p.S] = z;
-    z = fmaf(s == n - 1 ? last : full, z, share);
+  const double ld = (double)p.log_decay[head % p.H];
+  const float full = (float)exp(ld * p.seg_len), last = (float)exp(ld * (p.L - (n - 1) * p.seg_len));
+  for (int k0 = 0; k0 < n; k0 += AHEAD) {
+    float share[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = k0 + j;
+      share[j] = k < n - 1 ? part[(int64_t)(rev ? n - 1 - k : k) * p.S] : 0.f;      // nobody formed the last one's
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = k0 + j, s = rev ? n - 1 - k : k;
+      if (k < n) {
+        part[(int64_t)s * p.S] = z;
+        z = fmaf(s == n - 1 ? last : full, z, share[j]);
+      }
+    }
   }
 }
 
