@@ -16,8 +16,8 @@
 // accumulator and no operand is rounded twice.  That needs a^{-64} to stay far from overflow: heads with a < 1/2 (`steep`) keep
 // a^{t-s} on the scores, where it is at most 1, and their carried part is scaled row by row in TMEM before P v' joins it.
 //
-// What bounds it is shared-memory bandwidth (the MMAs' operands) and the power limit, so operands are kept out of shared memory
-// where TMEM can hold them: per chunk and head of 128 x 128 the tiles move 96 KB in, 288 KB to the MMAs and 160 KB for the element
+// What bounds it is the rate of the MMAs (48 of 128 x 128 x 16 a chunk: 107 cycles each with both operands in shared memory, 74 with
+// one in TMEM; 4100 of the 5600 cycles that a chunk takes) and the power limit, so operands are kept in TMEM where it can hold them: per chunk and head of 128 x 128 the tiles move 96 KB in, 288 KB to the MMAs and 160 KB for the element
 // passes.  (With the parts of f v' in shared memory and 64 channels a CTA it was 800 KB, and 158 us where it now takes 119.)
 // Measured: forward [8, 4096, 16, 128, 128] 114 to 119 us (4.5 to 4.7 TB/s of operands and output), backward 360 us; prompt
 // [1, 65536, 16, 128, 128] 341 us.  Random operands draw 1000 W and the SM clock falls to 1.4 to 1.6 GHz; zeros run 20% faster.
