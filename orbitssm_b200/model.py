@@ -114,8 +114,13 @@ class ResidualBlock(nn.Module):
         return self.mixer.validate_state(state, **kw)
 
 
+def _hooked(m):
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
 def _joins(block):
-    return getattr(block, "joins", False)
+    """Does the stack join the block's output to the stream itself?  (A block that somebody listens to is called as a module.)"""
+    return getattr(block, "joins", False) and not _hooked(block)
 
 
 class BlockStack(nn.Module):
@@ -152,9 +157,8 @@ class BlockStack(nn.Module):
 
     def _next_norm(self, i):
         """The norm that follows joining block i, where that block may form it: the next joining block's or the final one."""
-        if i + 1 == len(self.layers):
-            return self.norm_f
-        return self.layers[i + 1].norm if _joins(self.layers[i + 1]) else None
+        norm = self.norm_f if i + 1 == len(self.layers) else self.layers[i + 1].norm if _joins(self.layers[i + 1]) else None
+        return None if norm is None or _hooked(norm) else norm
 
     @property
     def ssm_layers(self):

@@ -173,6 +173,27 @@ def test_joined_blocks_beside_plain_ones_and_other_mixers():
         assert rel(got, want) < TOL
 
 
+def test_hooks_of_joined_blocks_and_norms_are_called():
+    torch.manual_seed(3)
+    stack = ob.BlockStack.from_mixers([mixer() for _ in range(3)], 64, post_norm=True, gate=True, residual_scale=0.5).to("cuda")
+    x = torch.randn(2, 40, 64, device="cuda")
+    with torch.no_grad():
+        want = stack(x)
+        seen = []
+        handles = [m.register_forward_hook(lambda m, i, o, n=n: seen.append(n)) for n, m in
+                   (("block 1", stack.layers[1]), ("norm 2", stack.layers[2].norm), ("final", stack.norm_f))]
+        got = stack(x)
+        assert seen == ["block 1", "norm 2", "final"]
+        # norms of the rounded stream instead of the unrounded one: three roundings of float32 of a stream that three blocks pass
+        assert rel(got, want) < 64 * 2.0 ** -24
+        y, state = stack(x, return_state=True)
+        assert rel(y, want) < 64 * 2.0 ** -24 and seen == ["block 1", "norm 2", "final"] * 2
+        stack.step(x[:, 0], state)
+        for h in handles:
+            h.remove()
+        assert torch.equal(stack(x), want)
+
+
 def test_autocast_keeps_a_float32_stream():
     torch.manual_seed(4)
     stack = ob.BlockStack.from_mixers([mixer(128, 2) for _ in range(2)], 128, post_norm=True, gate=True, residual_scale=0.5).to(DEV)
