@@ -12,6 +12,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -76,13 +77,11 @@ PyObject* result(int status, std::initializer_list<at::Tensor> outs, int launche
   return t;
 }
 
-#define GUARDED(...)                                         \
-  try {                                                      \
-    __VA_ARGS__                                              \
-  } catch (const std::exception& e) {                        \
-    PyErr_SetString(PyExc_RuntimeError, e.what());           \
-    return nullptr;                                          \
-  }
+// C++ exceptions become the Python ones that torch raises for them (an out-of-memory error stays one)
+#define GUARDED(...)   \
+  HANDLE_TH_ERRORS     \
+  __VA_ARGS__          \
+  END_HANDLE_TH_ERRORS
 
 // the state and the decays of a call: [B, H, Dv, Dk] and [H] float32, dense
 bool state_ok(const at::Tensor& s, int64_t B, int64_t H, int64_t Dv, int64_t Dk) {

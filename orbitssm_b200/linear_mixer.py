@@ -259,6 +259,8 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out_state=No
     if out_state is not None and out_state.data_ptr() != state.data_ptr() and _overlap(out_state, state):
         raise ValueError(f"{who}: out_state overlaps state without being it")
     new = torch.empty_like(state) if out_state is None else out_state
+    if out_state is not None and not out_state.is_inference():
+        torch.autograd.graph.increment_version(out_state)        # a graph that kept it must not read the new one
     y = like(v)
     if B:
         qb, qh, _ = q.stride()

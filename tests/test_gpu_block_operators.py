@@ -546,6 +546,33 @@ def test_block_norm_gradients_on_either_host_way_are_the_same_bits(dtype):
                 assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
 
 
+def test_a_state_written_in_place_is_seen_by_a_graph_that_kept_it():
+    q, k, v, ld, s0, _, _ = _inputs(1, 70, 2, 64, 64, F32, 44)
+    y = ob.linear_attention(q.requires_grad_(True), k, v, ld, s0)
+    with torch.no_grad():
+        ob.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s0, out_state=s0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        s = s0.clone()
+        z, new = ob.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s, out_state=s)
+        want, _ = ob.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s0)
+        assert new is s and torch.equal(z, want)
+
+
+def test_running_out_of_memory_keeps_its_type():
+    x = torch.zeros(1 << 22, 32, device=DEV, dtype=BF)                     # its codes would take 128 MB
+    torch.cuda.empty_cache()
+    free = torch.cuda.memory_reserved() + (64 << 20)
+    torch.cuda.set_per_process_memory_fraction(free / torch.cuda.get_device_properties(0).total_memory)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            ob.pack_activation(x)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert ob.pack_activation(x).q.shape == x.shape
+
+
 def test_calls_on_tensors_of_another_type_or_place_are_refused_on_the_gpu_too():
     q, k, v, ld, s0, _, _ = _inputs(1, 4, 2, 8, 8, F32, 42)
     with pytest.raises(ValueError, match="one dtype"):
