@@ -4,7 +4,8 @@
 //
 // One CTA owns (batch, head, segment) and walks the chunks of its segment:
 //   S1[t,s] = q'_t . k'_s                      128 x 128 x X   both operands as TMA wrote them
-//   P[t,s]  = S1[t,s] a^{c-s} (s <= t, else 0) -> bfloat16     the only rounding of the part inside the chunk
+//   P[t,s]  = S1[t,s] a^{c-s} (s <= t, else 0) -> bfloat16     the only rounding of the part inside the chunk (sequences
+//                                                              of at most 32 tokens: in two parts)
 //   O[t,e]  = P v' + q' Zb^T                   128 x E x (128 + X)   P read from TMEM; Zb = a^{c+1} s_in / s_out Z rounded to
 //                                                              bfloat16, the only rounding of that part
 //   dZ[e,x] = sum_s (f_s v'_s[e]) k'_s[x]      128 x X x 384   f_s v' in three bfloat16 parts (their sum is it to 2^-25),
@@ -132,6 +133,9 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3;
   const int s0 = seg * p.seg_len, s1 = min(p.L, s0 + p.seg_len), nch = (s1 - s0 + LT_T - 1) / LT_T;
   const int xblocks = X > 64 ? 2 : 1, eblocks = E > 64 ? 2 : 1;   // a narrow head's second blocks are never loaded nor read
+  // A sequence of one slab of 32 tokens: P's sums have too few terms for its roundings to average out, so it keeps the rest of the
+  // rounding as well, in the place of the next slab, which is empty (k-steps 2 and 3, over the same tokens).
+  const bool brief = !local && p.L <= 32;
   // The state-only launch has room for two accumulators of dZ in the places of S1 and O: the next product need not wait for the state.
   constexpr int SETS = local ? 2 : 1;
   auto dz_column = [](int c) { return local ? (uint32_t)(c & 1) * 128u : LT_DZ; };
@@ -246,7 +250,8 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
           const uint32_t bv = lo_mn(base(c, 4));
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) umma_bf16_ta_h(tbase + LT_O, tbase + LT_P + ks * 8, bv + inc_mn(ks), id_o, 1u);
+            for (int ks = 0; ks < 8; ++ks)
+              if (!brief || ks < 4) umma_bf16_ta_h(tbase + LT_O, tbase + LT_P + ks * 8, bv + (brief ? inc_mn(ks & 1) : inc_mn(ks)), id_o, 1u);
             umma_commit(&bars.p_empty);
             umma_commit(&bars.acc_full);
           }
@@ -309,6 +314,7 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
             if (rev ? j < q : j > q) {                       // wholly beyond the diagonal
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = 0u;
+              if (brief) tmem_st16(tmem_addr(tbase, q * 32, LT_P + 16), o);
             } else {
               uint32_t r[32];
               tmem_ld32(tmem_addr(tbase, q * 32, LT_S1 + j * 32), r);
@@ -338,8 +344,19 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
               }
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = pack_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+              if (brief) {
+                uint32_t rest[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  float lo, hi;
+                  unpack_bf16(o[i], lo, hi);
+                  rest[i] = pack_bf16(__uint_as_float(r[2 * i]) - lo, __uint_as_float(r[2 * i + 1]) - hi);
+                }
+                tmem_st16(tmem_addr(tbase, q * 32, LT_P + 16), rest);
+              }
             }
             tmem_st16(tmem_addr(tbase, q * 32, LT_P + j * 16), o);
+            if (brief) break;
           }
           tmem_st_wait();
         }

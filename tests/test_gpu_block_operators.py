@@ -243,6 +243,27 @@ def test_joined_segments_at_the_ends_of_the_decay_range(decay, dtype):
     _check_all(q, k, v, ld, s0, dy, ds1, dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_decays_on_either_side_of_one_half(dtype):
+    q, k, v, _, s0, dy, ds1 = _inputs(1, 700, 6, 96, 128, dtype, 54)
+    ld = torch.tensor([-0.1, -0.69314, -0.69316, -0.8, -2.0, -5.0], device=DEV)
+    _check_all(q, k, v, ld, s0, dy, ds1, dtype)
+
+
+@pytest.mark.parametrize("case", [(3, 1, 2, 96, 32), (2, 2, 1, 72, 128), (1, 17, 3, 64, 64), (2, 32, 2, 128, 128)])
+def test_short_sequences_are_rounded_once(case):
+    """Without a state, up to 32 tokens: scores in two bfloat16 parts, off by 2^-16, and their decays by 2^-17 at most."""
+    q, k, v, ld, _, dy, _ = _inputs(*case, BF, 55)
+    sc = case[3] ** -0.5
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    y = ob.linear_attention(*leaves, ld)
+    got = [y, *torch.autograd.grad(y, leaves, dy)]
+    zero = torch.zeros(case[0], case[2], case[4], case[3], device=DEV)
+    want, big = ref_attention(q, k, v, ld, None, sc, dy, zero), majorant(q, k, v, ld, None, sc, dy, zero)
+    for i, j in enumerate((0, 2, 3, 4)):
+        close(got[i], want[j], big[j], BF, 8 + 2 * 128 + 128, 2.0 ** -16 + 2.0 ** -17)
+
+
 def test_one_token_is_the_step():
     for dtype in (BF, F32):
         q, k, v, ld, s0, _, _ = _inputs(3, 1, 4, 72, 128, dtype, 53)
