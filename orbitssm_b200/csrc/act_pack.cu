@@ -158,10 +158,10 @@ __global__ void __launch_bounds__(PACK_THREADS) unpack_flat_kernel(const uint4* 
 }
 
 // Any width, any row stride: four lanes own a group, eight elements each, in accesses of W elements (8, 4, 2 or 1: what the width,
-// the row stride and the addresses allow) that the lanes take in turn, so that one access of the four lies side by side.  ROW_ITEMS groups a lane in flight.  Both directions of 67 million bfloat16
-// elements in rows of 1000: 91 us (4.5 TB/s; eight lanes of four elements took 109), of 250: 115 us; odd widths move single
-// bytes: 203 us in rows of 251.  Every lane of a warp takes part in the shuffles;
-// the ones past the end hold nothing.
+// the row stride and the addresses allow) that the lanes take in turn, so that one access of the four lies side by side.
+// ROW_ITEMS groups a lane in flight.  Both directions of 67 million bfloat16 elements in rows of 1000: 91 us (4.5 TB/s; eight lanes
+// of four elements took 109), of 250: 115 us; odd widths move single bytes: 203 us in rows of 251.  Every lane of a warp takes part
+// in the shuffles; the ones past the end hold nothing.
 constexpr int ROW_ITEMS = 2, LANE_ELEMS = 8, GROUP_LANES = PACK_GROUP / LANE_ELEMS;
 constexpr int ROW_GROUPS = PACK_THREADS / GROUP_LANES;                 // groups a block and item
 

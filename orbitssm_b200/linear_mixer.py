@@ -219,7 +219,8 @@ def linear_attention(q, k, v, log_decay, state=None, *, scale=None, return_state
 
     bfloat16 heads whose widths are multiples of 8 up to 128 run on tensor-core tiles: products of the unrounded inputs with the
     scores or the state rounded once to bfloat16 (scores of up to 32 tokens in two parts), float32 sums; the state itself is
-    float32 throughout.  Other calls run on float32 kernels.  Values are expected to be finite: a NaN or infinity may reach every output of its head and sequence."""
+    float32 throughout.  Other calls run on float32 kernels.  Values are expected to be finite: a NaN or infinity may reach every
+    output of its head and sequence."""
     if log_decay.requires_grad:
         _checked(q, k, v, log_decay, state, scale)               # refuses a gradient of it
     if wants_grad(q, k, v, state):
