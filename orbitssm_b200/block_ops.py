@@ -8,6 +8,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+import torch.utils.checkpoint
 
 from . import _lib, ops
 
@@ -305,39 +306,26 @@ def unpack_activation(packed, dtype=None):
     return x
 
 
-class CheckpointFn(torch.autograd.Function):
-    """``block(x)`` without keeping what the block's backward needs: its input waits in eight bits, and the backward pass
-    restores it, runs the block again and differentiates that run."""
-
-    @staticmethod
-    def forward(ctx, block, x, *params):
-        ctx.block = block
-        ctx.amp = (torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda"))
-        packed = pack_activation(x)
-        ctx.dtype = x.dtype
-        with torch.no_grad():
-            y = block(x)
-        ctx.save_for_backward(packed.q, packed.exponent, *params)     # the parameters: a change in place before the backward is refused
-        return y
-
-    @staticmethod
-    @ops.first_order_only("8-bit activation checkpoint")
-    def backward(ctx, dy):
-        q, e, *params = ctx.saved_tensors
-        x = unpack_activation(PackedActivation(q, e, ctx.dtype)).requires_grad_(ctx.needs_input_grad[1])
-        wanted = [p for p, need in zip(params, ctx.needs_input_grad[2:]) if need]
-        ins = ([x] if ctx.needs_input_grad[1] else []) + wanted
-        enabled, dtype = ctx.amp
-        with torch.enable_grad(), torch.autocast("cuda", dtype=dtype, enabled=enabled, cache_enabled=False):
-            y = ctx.block(x)
-        grads = list(torch.autograd.grad(y, ins, dy, allow_unused=True))
-        dx = grads.pop(0) if ctx.needs_input_grad[1] else None
-        return (None, dx, *[grads.pop(0) if need else None for need in ctx.needs_input_grad[2:]])
-
-
 def checkpoint_block(block, x):
-    """``block(x)`` under an 8-bit activation checkpoint (see `CheckpointFn`); an ordinary call where no gradient is wanted."""
-    params = [p for p in block.parameters() if p.requires_grad]
-    if not torch.is_grad_enabled() or not (x.requires_grad or params):
+    """``block(x)`` without keeping what the block's backward needs: its input waits in eight bits, and the backward pass restores
+    it, runs the block again from it and differentiates the block's own graph with what that run saves (so that hooks of parameters
+    and modules see one backward pass).  A parameter changed in place in between is refused.  An ordinary call where no gradient is
+    wanted."""
+    params = list(block.parameters())
+    if not torch.is_grad_enabled() or not (x.requires_grad or any(p.requires_grad for p in params)):
         return block(x)
-    return CheckpointFn.apply(block, x, *params)
+    packed = pack_activation(x)
+    dtype, wanted = x.dtype, x.requires_grad
+    versions = [(p, p._version) for p in params if not p.is_inference()]
+    first = [x]
+
+    def run(q, exponent):
+        if first:
+            return block(first.pop())
+        for p, version in versions:
+            if p._version != version:
+                raise RuntimeError(f"8-bit activation checkpoint: a parameter {tuple(p.shape)} that the block's backward pass needs was "
+                                   f"modified by an inplace operation (version {p._version}, expected {version})")
+        return block(unpack_activation(PackedActivation(q, exponent, dtype)).requires_grad_(wanted))
+
+    return torch.utils.checkpoint.checkpoint(run, packed.q, packed.exponent, use_reentrant=False, preserve_rng_state=False)

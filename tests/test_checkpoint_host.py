@@ -1,0 +1,116 @@
+"""CPU: the autograd side of 8-bit activation checkpoints, with the two kernels replaced by copies, so that a checkpointed block has
+to give what the block gives without one, bit for bit."""
+import pytest
+import torch
+import torch.nn as nn
+
+from orbitssm_b200 import block_ops
+
+
+@pytest.fixture(autouse=True)
+def copies(monkeypatch):
+    monkeypatch.setattr(block_ops, "pack_activation",
+                        lambda x: block_ops.PackedActivation(x.detach().clone(), x.new_zeros(1, dtype=torch.uint8), x.dtype))
+    monkeypatch.setattr(block_ops, "unpack_activation", lambda p, dtype=None: p.q.clone())
+
+
+def _block(seed=0):
+    torch.manual_seed(seed)
+    return nn.Sequential(nn.Linear(8, 8), nn.Tanh(), nn.Linear(8, 8)).double()
+
+
+def _x(seed=1):
+    return torch.randn(3, 8, generator=torch.Generator().manual_seed(seed), dtype=torch.float64).requires_grad_(True)
+
+
+def _grads(block, checkpointed, x):
+    params = list(block.parameters())
+    for t in (x, *params):
+        t.grad = None
+    y = block_ops.checkpoint_block(block, x) if checkpointed else block(x)
+    (y * torch.arange(8.0, dtype=y.dtype)).sum().backward()
+    return [y.detach(), x.grad, *[p.grad for p in params]]
+
+
+def _same(block, x):
+    return all(torch.equal(a, b) for a, b in zip(_grads(block, True, x), _grads(block, False, x), strict=True))
+
+
+def test_gradients_are_the_blocks_own():
+    assert _same(_block(), _x())
+
+
+def test_hooks_of_parameters_run_once():
+    block, x = _block(), _x()
+    calls = []
+    block[0].weight.register_hook(lambda g: calls.append(0) or 0.5 * g)
+    block[2].bias.register_post_accumulate_grad_hook(lambda p: calls.append(1))
+    assert _same(block, x) and sorted(calls) == [0, 0, 1, 1]            # once with the checkpoint, once without
+    block[0].weight.register_hook(lambda g: None)
+    g, = torch.autograd.grad(block_ops.checkpoint_block(block, x).sum(), block[0].weight)
+    want, = torch.autograd.grad(block(x).sum(), block[0].weight)
+    assert torch.equal(g, want)
+
+
+def test_hooks_of_modules_inside_the_block_run_in_the_backward_pass_once():
+    block, x = _block(), _x()
+    calls = []
+    block[1].register_full_backward_hook(lambda m, gi, go: calls.append(0))
+    assert _same(block, x) and calls == [0, 0]
+
+
+def test_a_parameter_that_the_block_reaches_by_another_way_keeps_its_gradient():
+    block, x = _block(), _x()
+
+    class Outer(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.inner = block
+            self.kept = [block[2].weight]                                # not looked up in the module at the time of the call
+
+        def forward(self, x):
+            return self.inner[1](x @ self.kept[0].t())
+
+    assert _same_or_none(Outer(), x)
+
+
+def _same_or_none(block, x):
+    return all((a is None) == (b is None) and (a is None or torch.equal(a, b))
+               for a, b in zip(_grads(block, True, x), _grads(block, False, x), strict=True))
+
+
+def test_a_change_of_a_parameter_before_the_backward_pass_is_refused():
+    block, x = _block(), _x()
+    y = block_ops.checkpoint_block(block, x)
+    with torch.no_grad():
+        block[0].weight.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    frozen = _block()
+    frozen[2].weight.requires_grad_(False)                               # the second run would read it as well
+    y = block_ops.checkpoint_block(frozen, x)
+    with torch.no_grad():
+        frozen[2].weight.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_a_kept_graph_is_walked_twice_and_the_input_may_change():
+    block, x = _block(), _x()
+    want = _grads(block, False, x)[1]
+    x2 = x.detach().clone().requires_grad_(True)
+    h = x2 * 1.0
+    y = (block_ops.checkpoint_block(block, h) * torch.arange(8.0, dtype=torch.float64)).sum()
+    h.data.zero_()                                                       # what waits for the backward pass is the packed copy
+    for _ in range(2):
+        g, = torch.autograd.grad(y, x2, retain_graph=True)
+        assert torch.equal(g, want)
+
+
+def test_nothing_is_recorded_without_a_gradient():
+    block, x = _block(), _x()
+    with torch.no_grad():
+        assert not block_ops.checkpoint_block(block, x).requires_grad
+    for p in block.parameters():
+        p.requires_grad_(False)
+    assert not block_ops.checkpoint_block(block, x.detach()).requires_grad
