@@ -5,6 +5,7 @@ C-ABI library on the current stream of the tensors' device.
 """
 from __future__ import annotations
 
+import weakref
 from typing import NamedTuple
 
 import torch
@@ -306,26 +307,72 @@ def unpack_activation(packed, dtype=None):
     return x
 
 
+#: block -> {the training flags of its modules: does it draw from the GPU's generator?}, as uncaptured runs have shown
+_DRAWS = weakref.WeakKeyDictionary()
+
+
+def _flags(block):
+    return tuple(m.training for m in block.modules())
+
+
+class _Drawn:
+    """What a block's first run drew: the second one draws the same, and leaves the generators (the CPU's and the one of the block's
+    device) as it found them."""
+
+    def __init__(self, block, device):
+        self.generators = [torch.default_generator]
+        if device.type == "cuda":
+            gpu = torch.cuda.default_generators[device.index]
+            if not torch.cuda.is_current_stream_capturing():
+                self.generators.append(gpu)
+            else:
+                # inside a capture a generator cannot be set back
+                draws = _DRAWS.get(block, {}).get(_flags(block))
+                if draws is None:
+                    raise RuntimeError("8-bit activation checkpoint: run the block forward once, in the mode it is to be captured in, before "
+                                       "the capture: only such a run shows whether it draws random numbers")
+                if draws:
+                    raise RuntimeError("8-bit activation checkpoint: a block that draws random numbers on the GPU cannot be captured into a "
+                                       "graph: its second run would draw others than its first")
+        self.states = [g.get_state() for g in self.generators]
+
+    def note(self, block):
+        if len(self.generators) == 2:
+            _DRAWS.setdefault(block, {})[_flags(block)] = not torch.equal(self.generators[1].get_state(), self.states[1])
+
+    def __enter__(self):
+        self.found = [g.get_state() for g in self.generators]
+        for g, s in zip(self.generators, self.states):
+            g.set_state(s)
+
+    def __exit__(self, *exc):
+        for g, s in zip(self.generators, self.found):
+            g.set_state(s)
+
+
 def checkpoint_block(block, x):
     """``block(x)`` without keeping what the block's backward needs: its input waits in eight bits, and the backward pass restores
     it, runs the block again from it and differentiates the block's own graph with what that run saves (so that hooks of parameters
-    and modules see one backward pass).  A parameter changed in place in between is refused.  An ordinary call where no gradient is
-    wanted."""
+    and modules see one backward pass).  The second run draws the random numbers of the first.  Refused: a parameter changed in
+    place in between, and a block that draws on the GPU inside a graph capture.  An ordinary call where no gradient is wanted."""
     params = list(block.parameters())
     if not torch.is_grad_enabled() or not (x.requires_grad or any(p.requires_grad for p in params)):
         return block(x)
     packed = pack_activation(x)
     dtype, wanted = x.dtype, x.requires_grad
     versions = [(p, p._version) for p in params if not p.is_inference()]
-    first = [x]
+    first, drawn = [x], _Drawn(block, x.device)
 
     def run(q, exponent):
         if first:
-            return block(first.pop())
+            y = block(first.pop())
+            drawn.note(block)
+            return y
         for p, version in versions:
             if p._version != version:
                 raise RuntimeError(f"8-bit activation checkpoint: a parameter {tuple(p.shape)} that the block's backward pass needs was "
                                    f"modified by an inplace operation (version {p._version}, expected {version})")
-        return block(unpack_activation(PackedActivation(q, exponent, dtype)).requires_grad_(wanted))
+        with drawn:
+            return block(unpack_activation(PackedActivation(q, exponent, dtype)).requires_grad_(wanted))
 
     return torch.utils.checkpoint.checkpoint(run, packed.q, packed.exponent, use_reentrant=False, preserve_rng_state=False)

@@ -147,7 +147,8 @@ class BlockStack(nn.Module):
         """``"int8"``: a training forward keeps of each block its input alone, in eight bits an element (`pack_activation`), and the
         backward pass runs the block again from it; None: every block keeps what its backward needs.  The gradients are then those of
         the blocks at the restored inputs (off by at most 1/128 of the largest of each 32 channels).  Outputs do not change.  Calls
-        with a state, or that return one, keep everything as without it."""
+        with a state, or that return one, keep everything as without it.  A block that draws random numbers draws the same ones when
+        it runs again; captured into a graph it is refused."""
         if mode not in (None, "int8"):
             raise ValueError(f"set_checkpoint: mode must be None or 'int8', got {mode!r}")
         if mode is not None and any(getattr(m, "_cp", None) is not None for m in self.ssm_layers):

@@ -114,3 +114,26 @@ def test_nothing_is_recorded_without_a_gradient():
     for p in block.parameters():
         p.requires_grad_(False)
     assert not block_ops.checkpoint_block(block, x.detach()).requires_grad
+
+
+class Drop(nn.Module):
+    """A mixer's dropout, by the function: nothing in the module tells that it draws."""
+
+    def __init__(self, p=0.5):
+        super().__init__()
+        self.lin, self.p = nn.Linear(8, 8).double(), p
+
+    def forward(self, x):
+        return nn.functional.dropout(self.lin(x), self.p, self.training)
+
+
+def test_random_numbers_are_drawn_again_as_they_were():
+    torch.manual_seed(5)
+    block, x = Drop(), torch.randn(64, 8, dtype=torch.float64, requires_grad=True)
+    y = block_ops.checkpoint_block(block, x)
+    after = torch.get_rng_state()
+    gb, gx = torch.autograd.grad(y.sum(), (block.lin.bias, x))
+    assert torch.equal(torch.get_rng_state(), after)                     # the backward pass leaves the generator as it was
+    kept = (y.detach() != 0).double()
+    assert torch.equal(gb, (2.0 * kept).sum(0))
+    assert torch.allclose(gx, (2.0 * kept) @ block.lin.weight.detach(), rtol=1e-14, atol=0)

@@ -4,6 +4,7 @@ import torch
 
 import orbitssm_b200 as ob
 from orbitssm_b200 import ops
+from orbitssm_b200.block_ops import checkpoint_block
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -34,3 +35,45 @@ def test_a_hook_of_a_parameter_runs_once(kw):
     got = grads()
     assert len(calls) == len(want) and all(torch.equal(a, 0.5 * b) for a, b in zip(got, want))
     ops.check_device_status()
+
+
+class DropMixer(torch.nn.Module):
+    """A mixer of plain modules that draws from the GPU's generator."""
+
+    def __init__(self, d=64):
+        super().__init__()
+        self.lin = torch.nn.Linear(d, d)
+
+    def forward(self, x):
+        return torch.nn.functional.dropout(self.lin(x), 0.5, self.training)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(residual_scale=1.0)])
+def test_a_mixer_that_draws_random_numbers(kw):
+    torch.manual_seed(4)
+    block = ob.BlockStack.from_mixers([DropMixer()], 64, **kw).to(DEV).layers[0]
+    x = torch.randn(4, 30, 64, device=DEV)
+    seen = []
+    block.mixer.register_forward_hook(lambda m, i, o: seen.append(o.detach().clone()))
+    y = checkpoint_block(block, x)
+    after = torch.cuda.get_rng_state()
+    g, = torch.autograd.grad(y.sum(), block.mixer.lin.bias)
+    assert torch.equal(torch.cuda.get_rng_state(), after)
+    assert bool((seen[0] == 0).any()) and torch.equal(g, (2.0 * (seen[0] != 0)).sum((0, 1)))    # whole numbers: exact
+
+
+def test_a_block_that_draws_is_not_captured():
+    def stack(training):
+        torch.manual_seed(4)
+        return ob.BlockStack.from_mixers([DropMixer()], 64).to(DEV).set_checkpoint("int8").train(training)
+
+    x = torch.randn(4, 30, 64, device=DEV)
+    with pytest.raises(ob.CaptureError, match="draws random numbers"):
+        ob.GraphedStep(stack(True), x, x)
+    quiet = stack(False)                                                 # the same block, drawing nothing in this mode
+    step = ob.GraphedStep(quiet, x, x)
+    with torch.no_grad():
+        assert torch.equal(step(x, x), quiet(x))
+    fresh = stack(False)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()), pytest.raises(RuntimeError, match="before the capture"):
+        fresh(x)
