@@ -10,6 +10,7 @@ from typing import NamedTuple
 
 import torch
 import torch.utils.checkpoint
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 
@@ -53,8 +54,8 @@ def launch(name, launches, device, fn, *args):
 
 def native(name, *args):
     """The outputs of host call `name` (`_lib.host`), or None where it leaves the call to the Python way."""
-    if ops._TIMING is not None:
-        return None                    # a timed region needs the events around the launch
+    if ops._TIMING is not None or forward_ad._current_level >= 0 or tracing():
+        return None                    # a timed region needs the events around the launch, the others the checks of the Python way
     got = getattr(_lib._host or _lib.host(), name)(*args)
     if got is None:
         return None
@@ -65,14 +66,34 @@ def native(name, *args):
     return outs
 
 
-def wants_grad(*tensors):
-    """Is a gradient recorded for any of them?  Where none is, a call skips the autograd node (about 10 us of host time)."""
+def tracing():
+    """Is `torch.jit.trace` recording?  A call that is no autograd node would be recorded as its empty outputs."""
+    return torch._C._get_tracing_state() is not None
+
+
+def not_traced(who):
+    if tracing():
+        raise RuntimeError(f"{who}: cannot be recorded by torch.jit.trace (it is not an autograd node)")
+
+
+def differentiated(*tensors):
+    """Is a gradient of any of them recorded, or does one carry a forward-mode tangent?"""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
     if not torch.is_grad_enabled():
         return False
     for t in tensors:
         if t is not None and t.requires_grad:
             return True
     return False
+
+
+def wants_node(*tensors):
+    """Does a call on them go through its autograd node?  Where it is differentiated (the node refuses forward mode) and under
+    `torch.jit.trace`.  Elsewhere a call skips the node (about 10 us of host time)."""
+    return tracing() or differentiated(*tensors)
 
 
 def same_device(who, dev, *tensors):
@@ -239,7 +260,7 @@ def block_norm(x, h, *, gate=None, scale=None, post_weight=None, pre_weight=None
     if not eps >= 0:
         raise ValueError(f"{who}: eps must be at least 0, got {eps!r}")
     same_device(who, x.get_device(), x, h, gate, scale, post_weight, pre_weight)
-    if not wants_grad(x, h, gate, scale, post_weight, pre_weight):
+    if not wants_node(x, h, gate, scale, post_weight, pre_weight):
         return _block_norm(x, h, gate, scale, post_weight, pre_weight, float(eps), False)[:2]
     return BlockNormFn.apply(x, h, gate, scale, post_weight, pre_weight, float(eps))
 
@@ -268,6 +289,7 @@ def pack_activation(x):
     if got is not None:
         return PackedActivation(*got, x.dtype)
     who = "pack_activation"
+    not_traced(who)
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"{who}: expected x [..., D] with D > 0, got {tuple(x.shape)}")
     code = io_code(who, x)
@@ -287,6 +309,7 @@ def pack_activation(x):
 def unpack_activation(packed, dtype=None):
     """The activation a `PackedActivation` stands for, in `dtype` (default: its own; exact in float32 and in bfloat16)."""
     who = "unpack_activation"
+    not_traced(who)
     q, e, own_dtype = packed
     dtype = own_dtype if dtype is None else dtype
     if dtype not in _DT:

@@ -18,7 +18,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, ops
-from .block_ops import io_code, launch, like, native, same_device, wants_grad
+from .block_ops import differentiated, io_code, launch, like, native, not_traced, same_device, wants_node
 from .config import BACKENDS, PRECISIONS, _positive_int, _strict_from_dict, as_execution
 from .state import State, StateLifecycle
 
@@ -185,7 +185,7 @@ def _check_operands(who, q, k, v, log_decay, state, lead):
         raise NotImplementedError(f"{who}: at least one head, of widths 1..256, got H={H} Dk={Dk} Dv={Dv}")
     if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
         raise ValueError(f"{who}: log_decay must be float32 [{H}], got {log_decay.dtype} {tuple(log_decay.shape)}")
-    if log_decay.requires_grad and torch.is_grad_enabled():
+    if differentiated(log_decay):
         raise ValueError(f"{who}: log_decay is a constant of the layer; its gradient is not served (detach it)")
     if state is not None and (state.shape != (B, H, Dv, Dk) or state.dtype != torch.float32):
         raise ValueError(f"{who}: state must be float32 {(B, H, Dv, Dk)}, got {state.dtype} {tuple(state.shape)}")
@@ -221,9 +221,9 @@ def linear_attention(q, k, v, log_decay, state=None, *, scale=None, return_state
     scores or the state rounded once to bfloat16 (scores of up to 32 tokens in two parts), float32 sums; the state itself is
     float32 throughout.  Other calls run on float32 kernels.  Values are expected to be finite: a NaN or infinity may reach every
     output of its head and sequence."""
-    if log_decay.requires_grad:
+    if differentiated(log_decay):
         _checked(q, k, v, log_decay, state, scale)               # refuses a gradient of it
-    if wants_grad(q, k, v, state):
+    if wants_node(q, k, v, state):
         y, new = LinearAttentionFn.apply(q, k, v, log_decay, state, scale, bool(return_state), _slots)
         return (y, new) if return_state else y
     got = native("la_fwd", q, k, v, log_decay, state, scale, return_state)
@@ -243,10 +243,11 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out_state=No
         if got is not None:
             return tuple(got)
     who = "linear_attention_step"
+    not_traced(who)
     if state is None:
         raise ValueError(f"{who}: a state is required (zeros before the first token)")
     code = _check_operands(who, q, k, v, log_decay, state, ("B",))
-    if wants_grad(q, k, v, state):
+    if differentiated(q, k, v, state):
         raise ValueError(f"{who}: gradients are not served; use linear_attention on a sequence of one token, or torch.no_grad()")
     if out_state is not None and (out_state.shape != state.shape or out_state.dtype != torch.float32 or not out_state.is_contiguous()
                                   or out_state.device != state.device):
