@@ -30,6 +30,17 @@ class RMSNorm(nn.Module):
         return ops.GateNormFn.apply(x, None, self.weight, self.eps)
 
 
+def _listened(m):
+    """Does somebody listen to calls of the module (its hooks, or hooks of every module)?"""
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks) or nn.modules.module._has_any_global_hook()
+
+
+def _plain(m, cls):
+    """Is `m` an ordinary `cls` whose arithmetic a kernel may do from its parameters?  (A subclass, a wrapper, another module in its place
+    and one that is listened to are called.)"""
+    return type(m) is cls and "forward" not in m.__dict__ and not _listened(m)
+
+
 class ResidualBlock(nn.Module):
     """``x + mixer(norm(x))``; with `post_norm`, `gate` or `residual_scale`
 
@@ -57,17 +68,22 @@ class ResidualBlock(nn.Module):
 
     def join(self, x, n, h, next_norm=None):
         """(x + scale * post_norm(h) * sigmoid(gate_proj(n)), next_norm of it | None) in one kernel."""
-        dt = torch.promote_types(x.dtype, h.dtype)          # as in x + h: under autocast a float32 stream stays float32
-        gate = None
+        gate, io = None, h.dtype
         if self.gate_proj is not None:
-            with torch.autocast("cuda", enabled=False):
-                gate = ops.ProjectFn.apply(n.to(h.dtype), None, 0, None, 0, self.gate_proj.weight).to(dt)
+            if _plain(self.gate_proj, nn.Linear) and self.gate_proj.bias is None:
+                with torch.autocast("cuda", enabled=False):
+                    gate = ops.ProjectFn.apply(n.to(io), None, 0, None, 0, self.gate_proj.weight)
+            else:
+                gate = self.gate_proj(n)
+        post = self.post_norm
+        if post is not None and not _plain(post, RMSNorm):
+            h, post = post(h), None
+        dt = torch.promote_types(x.dtype, h.dtype)          # as in x + h: under autocast a float32 stream stays float32
         # two norms of unlike eps are not one kernel's: the next norm then runs by itself
-        fused = next_norm if (next_norm is not None and (self.post_norm is None or next_norm.eps == self.post_norm.eps)) else None
-        eps = fused.eps if fused is not None else self.norm.eps if self.post_norm is None else self.post_norm.eps
-        r, out = block_norm(x.to(dt), h.to(dt), gate=gate, scale=self.scale,
-                            post_weight=None if self.post_norm is None else self.post_norm.weight,
-                            pre_weight=None if fused is None else fused.weight, eps=eps)
+        fused = next_norm if next_norm is not None and _plain(next_norm, RMSNorm) and (post is None or next_norm.eps == post.eps) else None
+        eps = fused.eps if fused is not None else 0.0 if post is None else post.eps
+        r, out = block_norm(x.to(dt), h.to(dt), gate=None if gate is None else gate.to(dt), scale=self.scale,
+                            post_weight=None if post is None else post.weight, pre_weight=None if fused is None else fused.weight, eps=eps)
         if next_norm is not None and fused is None:
             out = next_norm(r)
         return r, out
@@ -114,13 +130,11 @@ class ResidualBlock(nn.Module):
         return self.mixer.validate_state(state, **kw)
 
 
-def _hooked(m):
-    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
-
-
 def _joins(block):
-    """Does the stack join the block's output to the stream itself?  (A block that somebody listens to is called as a module.)"""
-    return getattr(block, "joins", False) and not _hooked(block)
+    """Does the stack join the block's output to the stream itself?  (A block of its own forward or step, and one that somebody listens
+    to, is called as a module.)"""
+    return getattr(block, "joins", False) and type(block).forward is ResidualBlock.forward and type(block).step is ResidualBlock.step \
+        and not {"forward", "step"} & block.__dict__.keys() and not _listened(block)
 
 
 class BlockStack(nn.Module):
@@ -158,8 +172,7 @@ class BlockStack(nn.Module):
 
     def _next_norm(self, i):
         """The norm that follows joining block i, where that block may form it: the next joining block's or the final one."""
-        norm = self.norm_f if i + 1 == len(self.layers) else self.layers[i + 1].norm if _joins(self.layers[i + 1]) else None
-        return None if norm is None or _hooked(norm) else norm
+        return self.norm_f if i + 1 == len(self.layers) else self.layers[i + 1].norm if _joins(self.layers[i + 1]) else None
 
     @property
     def ssm_layers(self):
