@@ -165,10 +165,14 @@ class BlockStack(nn.Module):
         it runs again; captured into a graph it is refused."""
         if mode not in (None, "int8"):
             raise ValueError(f"set_checkpoint: mode must be None or 'int8', got {mode!r}")
-        if mode is not None and any(getattr(m, "_cp", None) is not None for m in self.ssm_layers):
-            raise ValueError("set_checkpoint: blocks that run context-parallel are not checkpointed (their exchanges would run twice)")
+        if mode is not None:
+            self._refuse_context_parallel()
         self.checkpoint = mode
         return self
+
+    def _refuse_context_parallel(self):
+        if any(getattr(m, "_cp", None) is not None for m in self.layers.modules()):
+            raise ValueError("set_checkpoint: blocks that run context-parallel are not checkpointed (their exchanges would run twice)")
 
     def _next_norm(self, i):
         """The norm that follows joining block i, where that block may form it: the next joining block's or the final one."""
@@ -210,6 +214,7 @@ class BlockStack(nn.Module):
     def forward(self, x, state=None, return_state=False):
         if state is None and not return_state:
             if self.checkpoint is not None and torch.is_grad_enabled():
+                self._refuse_context_parallel()             # (it may have been switched on since)
                 for b in self.layers:
                     x = checkpoint_block(b, x)
                 return self.norm_f(x)

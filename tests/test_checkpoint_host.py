@@ -137,3 +137,26 @@ def test_random_numbers_are_drawn_again_as_they_were():
     kept = (y.detach() != 0).double()
     assert torch.equal(gb, (2.0 * kept).sum(0))
     assert torch.allclose(gx, (2.0 * kept) @ block.lin.weight.detach(), rtol=1e-14, atol=0)
+
+
+def test_blocks_that_run_context_parallel_are_refused_whenever_they_were_made_so():
+    import orbitssm_b200 as ob
+
+    class Mix(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.inner = nn.Linear(8, 8)
+
+        def forward(self, x):
+            raise AssertionError("the block ran")
+
+    stack = ob.BlockStack.from_mixers([Mix(), Mix()], 8).set_checkpoint("int8")
+    stack.layers[1].mixer._cp = object()                                 # what set_context_parallel leaves on a mixer
+    with pytest.raises(ValueError, match="context-parallel"):
+        stack(torch.zeros(2, 3, 8))
+    stack.layers[1].mixer._cp, stack.layers[0].mixer.inner._cp = None, object()
+    with pytest.raises(ValueError, match="context-parallel"):
+        stack(torch.zeros(2, 3, 8))
+    with pytest.raises(ValueError, match="context-parallel"):
+        stack.set_checkpoint("int8")
+    assert stack.set_checkpoint(None).checkpoint is None
