@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "liborbit_b200.so")
@@ -178,16 +179,30 @@ _HOST_ENTRIES = ("orbit_la_step", "orbit_la_fwd", "orbit_la_bwd", "orbit_la_work
                  "orbit_block_norm_bwd_workspace_bytes", "orbit_act_pack", "orbit_act_unpack")
 
 
+class _PythonSide:
+    """Stands for a host-call module that cannot be loaded: it leaves every call to the Python way."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def host():
-    """The native host calls of the block operators (``csrc/host_calls.cpp``), bound to this library's entry points."""
+    """The native host calls of the block operators (``csrc/host_calls.cpp``), bound to this library's entry points.  Without the module,
+    or with one that was built for another torch or Python, the Python way serves every call (same kernels, more host time): a warning
+    says so once."""
     global _host
     if _host is None:
         lib = load()
         try:
+            from . import build
+            if not build.host_matches():
+                raise ImportError("it was built for another torch or Python")
             from . import _orbit_host
-        except ImportError as e:
-            raise OrbitLibraryError(f"the extension module _orbit_host cannot be loaded ({e}): build it with "
-                                    "`python -m orbitssm_b200.build`") from e
+        except (ImportError, OSError) as e:
+            warnings.warn(f"the extension module _orbit_host cannot be loaded ({e}); the block operators take more host time.  Build it with "
+                          "`python -m orbitssm_b200.build`", RuntimeWarning, stacklevel=3)
+            _host = _PythonSide()
+            return _host
         _orbit_host.bind(*[C.cast(getattr(lib, n), C.c_void_p).value for n in _HOST_ENTRIES])
         _host = _orbit_host
     return _host

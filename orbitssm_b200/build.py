@@ -2,7 +2,8 @@
 
 Each ``csrc/*.cu`` is compiled to an object file under ``csrc/_obj`` (in parallel, and only when it or a header is newer
 than its object), then the objects are linked into the shared library next to this file.  ``csrc/host_calls.cpp`` (host code
-against the headers of the installed torch, no kernels) becomes the extension module ``_orbit_host.so`` beside it."""
+against the headers of the installed torch, no kernels) becomes the extension module ``_orbit_host.so`` beside it; where it cannot be
+built the library stands by itself, and the operators' Python host side serves every call."""
 from __future__ import annotations
 
 import glob
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -44,9 +46,22 @@ def stale() -> bool:
     return _newer(OUT, sources() + headers())
 
 
+def host_tag() -> str:
+    """What the host-call module is built against: its C++ ABI is the one of this torch and this Python alone."""
+    import torch
+    return f"orbit_host for torch {torch.__version__}, Python {sys.version_info.major}.{sys.version_info.minor};"
+
+
+def host_matches() -> bool:
+    """Does the built module carry the tag of the running torch and Python?"""
+    with open(HOST_OUT, "rb") as f:
+        return host_tag().encode() in f.read()
+
+
 def build_host(force: bool = False) -> str:
     """The host-call extension (C++ against torch's headers; the torch libraries are found when the module is loaded)."""
-    if not force and not _newer(HOST_OUT, [HOST_SRC, os.path.join(os.path.dirname(HERE), "include", "orbit_b200.h")]):
+    header = os.path.join(os.path.dirname(HERE), "include", "orbit_b200.h")
+    if not force and not _newer(HOST_OUT, [HOST_SRC, header]) and host_matches():
         return HOST_OUT
     import sysconfig
 
@@ -57,7 +72,7 @@ def build_host(force: bool = False) -> str:
     inc = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            os.path.join(cuda, "include")]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *["-I" + i for i in inc], HOST_SRC, "-o", HOST_OUT, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch",
+           f'-DORBIT_HOST_TAG="{host_tag()}"', *["-I" + i for i in inc], HOST_SRC, "-o", HOST_OUT, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch",
            "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
@@ -66,9 +81,17 @@ def build_host(force: bool = False) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    build_host(force)
-    if not force and not stale():
-        return OUT
+    if force or stale():
+        build_library(force, verbose)
+    try:
+        build_host(force)
+    except (RuntimeError, OSError, ImportError) as e:
+        warnings.warn(f"the native host calls were not built, the Python host side of the operators serves every call: {e}", RuntimeWarning, stacklevel=2)
+    return OUT
+
+
+def build_library(force: bool = False, verbose: bool = False) -> None:
+    """The C-ABI library; needs nvcc alone."""
     nvcc = os.environ.get("NVCC", "nvcc")
     os.makedirs(OBJ, exist_ok=True)
     hdrs = headers()
@@ -89,7 +112,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
     res = subprocess.run(link, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("link failed:\n" + " ".join(link) + "\n" + res.stdout + res.stderr)
-    return OUT
 
 
 if __name__ == "__main__":

@@ -362,7 +362,7 @@ PyObject* bind_status(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {METHOD("bind", bind),     METHOD("la_step", la_step), METHOD("la_fwd", la_fwd), METHOD("block_norm", block_norm),
                          METHOD("pack", pack),     METHOD("unpack", unpack),
                          METHOD("bind_status", bind_status), METHOD("la_bwd", la_bwd), METHOD("block_norm_bwd", block_norm_bwd), {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_orbit_host", "Native host calls of the block operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_orbit_host", "Native host calls of the block operators. " ORBIT_HOST_TAG, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

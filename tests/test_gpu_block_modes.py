@@ -67,3 +67,20 @@ def test_a_trace_holds_the_operators_or_is_refused():
     p = ob.pack_activation(x)
     with pytest.raises(RuntimeError, match="unpack_activation: cannot be recorded"):
         torch.jit.trace(lambda q: ob.unpack_activation(ob.PackedActivation(q, p.exponent, x.dtype)), (p.q,))
+
+
+def test_without_the_host_call_module_the_results_are_the_same_bits(monkeypatch):
+    from orbitssm_b200 import _lib
+    q, k, v, ld, s, x, w = _args(200)
+
+    def run():
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v, s, x, w)]
+        y, new = ob.linear_attention(*leaves[:3], ld, leaves[3], return_state=True)
+        r, n = ob.block_norm(leaves[4], leaves[4], gate=leaves[4], pre_weight=leaves[5])
+        out = [y, new, r, n, *torch.autograd.grad((y.sum() + new.sum() + (r * n).sum()), leaves)]
+        with torch.no_grad():
+            return out + [*ob.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s), ob.unpack_activation(ob.pack_activation(x))]
+
+    want = run()
+    monkeypatch.setattr(_lib, "_host", _lib._PythonSide())
+    assert all(torch.equal(a, b) for a, b in zip(run(), want, strict=True))
