@@ -160,8 +160,11 @@ class BlockStack(nn.Module):
     def set_checkpoint(self, mode):
         """``"int8"``: a training forward keeps of each block its input alone, in eight bits an element (`pack_activation`), and the
         backward pass runs the block again from it; None: every block keeps what its backward needs.  The gradients are then those of
-        the blocks at the restored inputs (off by at most 1/128 of the largest of each 32 channels).  Outputs do not change.  Calls
-        with a state, or that return one, keep everything as without it.  A block that draws random numbers draws the same ones when
+        the blocks at the restored inputs (off by at most 1/127 of the largest of each 32 channels).  Blocks run one after another, each
+        taking its norm from the stream as it is stored: outputs are those of the blocks called one by one, bit for bit.  That is also
+        what a stack of plain blocks gives without the mode; in a stack of joining blocks the ordinary call forms each norm from the
+        stream before its rounding, so that there outputs differ by that rounding (in bfloat16 2^-8 of each element before a norm).
+        Calls with a state, or that return one, keep everything as without it.  A block that draws random numbers draws the same ones when
         it runs again; captured into a graph it is refused."""
         if mode not in (None, "int8"):
             raise ValueError(f"set_checkpoint: mode must be None or 'int8', got {mode!r}")

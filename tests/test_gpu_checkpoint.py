@@ -77,3 +77,20 @@ def test_a_block_that_draws_is_not_captured():
     fresh = stack(False)
     with torch.cuda.graph(torch.cuda.CUDAGraph()), pytest.raises(RuntimeError, match="before the capture"):
         fresh(x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_outputs_with_and_without_the_checkpoint(dtype):
+    torch.manual_seed(6)
+    x = torch.randn(2, 70, 64, device=DEV, dtype=dtype)
+    plain = ob.BlockStack.from_mixers([mixer() for _ in range(3)], 64).to(DEV).to(dtype)
+    want = plain(x).detach()
+    assert torch.equal(plain.set_checkpoint("int8")(x).detach(), want)
+    # a joining block: the final norm is taken from the stream before or after its rounding.  That moves every element by u at most,
+    # relative to itself, so the root of the mean square by u as well, and either result is rounded once: 4 u, and terms of u^2
+    joined = ob.BlockStack.from_mixers([mixer()], 64, post_norm=True, gate=True, residual_scale=0.5).to(DEV).to(dtype)
+    want = joined(x).detach().double()
+    got = joined.set_checkpoint("int8")(x).detach().double()
+    u = torch.finfo(dtype).eps / 2
+    # (float32: the sum of the 64 squares and the product with the weight add their own roundings, fewer than 64)
+    assert bool(((got - want).abs() <= (4.1 * u + 64 * 2.0 ** -24) * want.abs()).all())
