@@ -282,9 +282,9 @@ class PackedActivation(NamedTuple):
 def pack_activation(x):
     """x [..., D] (float32 or bfloat16, a dense last axis) -> `PackedActivation`: a signed byte an element and one power of
     two for each 32 elements of a row, the least under which the group's largest element rounds to at most 127 (never below
-    2^-126).  Rounding is to nearest, ties to even: off by at most half a step, and a step is at most 1/64 of the group's
-    largest element (values within 2^122 of the type's largest are off by up to a step, so as to stay finite).  A non-finite
-    element is restored as NaN and leaves its group's scale alone.  Not differentiable."""
+    2^-126).  Rounding is to nearest, ties to even: off by at most half a step, that is 1/127.5 of the group's largest element
+    (2^-127 where that is more: a step is never below 2^-126; values within 2^122 of the type's largest are off by up to a step, so as
+    to stay finite).  A non-finite element is restored as NaN and leaves its group's scale alone.  Not differentiable."""
     got = native("pack", x)
     if got is not None:
         return PackedActivation(*got, x.dtype)

@@ -4,15 +4,17 @@
 //   e = the least exponent in [-126, 122] with round(amax 2^-e) <= 127,   q = round_to_even(x 2^-e),   x^ = q 2^e
 //
 // The scale is a power of two, so x 2^-e is exact and the only rounding is the one to the whole number q: at most half a step,
-// 2^(e-1), that is 2^-7 of the group's largest element or less.  x^ has seven significant bits: exact in bfloat16 as in
-// float32, and packing x^ again gives the same bytes.  e needs no division or logarithm: with amax = m 2^E, m in [1, 2), it is
-// E - 6, or E - 5 where 64 m would round to 128.  A step below 2^-126 is not taken (the restored values stay normal numbers).
-// Codes of the largest step (2^122) end at 63, so that x^ stays finite at the type's largest values (there off by one step at
-// most).  A non-finite element takes the code -128, which nothing else uses, and is restored as NaN; it does not enter amax, so its
+// 2^(e-1).  A step smaller by half would round amax to 128 or more, so amax >= 63.75 steps and the error is at most amax / 127.5
+// (reached: of a group whose largest is 127.5, the element 1 is restored as 0).  x^ has seven significant bits: exact in bfloat16
+// as in float32.  e needs no division or logarithm: with amax = m 2^E, m in [1, 2), it is E - 6, or E - 5 where 64 m would round to 128.
+// A step below 2^-126 is not taken (the restored values stay normal numbers; the error there is at most 2^-127, whatever amax).  Codes of the
+// largest step (2^122) end at 63, so that x^ stays finite at the type's largest values (there off by one step at most).  Packing x^
+// again restores the same values; the bytes are the same too, except at the largest step (codes of 63 come back as 126 of half of it).
+// A non-finite element takes the code -128, which nothing else uses, and is restored as NaN; it does not enter amax, so its
 // neighbours keep their precision.
 //
 // HBM-bound: es + 1 + 1/32 bytes an element in either direction; 16-byte accesses on both sides where rows allow.  Both directions
-// of 67 million elements in rows of 1024: bfloat16 72 us (5.6 TB/s), float32 131 us (5.1 TB/s).
+// of 67 million elements in rows of 1024: bfloat16 72 us (5.7 TB/s), float32 121 us (5.6 TB/s).
 #include "common.cuh"
 #include "../../include/orbit_b200.h"
 
@@ -84,9 +86,9 @@ __device__ __forceinline__ float value_of(uint32_t w_flipped, int k, float scale
   return f == -128.f ? __uint_as_float(0x7fffffffu) : f * scale;
 }
 
-// Rows that are whole numbers of groups and lie one after another: the array is a flat run of groups (67 million bfloat16 elements:
-// pack 42 us, unpack 39; by rows, as below, 53 and 46).  A thread owns 16
-// elements (half a group, one shuffle for the maximum), so that every access is 16 bytes wide; ITEMS of them in flight.
+// Rows that are whole numbers of groups and lie one after another: the array is a flat run of groups (67 million bfloat16 elements
+// in rows of 1024: pack 37 us, unpack 35; by rows, as below, in rows of 1000: 49 and 41).  A thread owns 16 elements (half a
+// group, one shuffle for the maximum), so that every access is 16 bytes wide; ITEMS of them in flight.
 template <typename T, int ITEMS>
 __global__ void __launch_bounds__(PACK_THREADS) pack_flat_kernel(const T* __restrict__ x, uint4* __restrict__ q,
                                                                  uint8_t* __restrict__ e, int64_t n16) {
@@ -159,13 +161,14 @@ __global__ void __launch_bounds__(PACK_THREADS) unpack_flat_kernel(const uint4* 
 
 // Any width, any row stride: four lanes own a group, eight elements each, in accesses of W elements (8, 4, 2 or 1: what the width,
 // the row stride and the addresses allow) that the lanes take in turn, so that one access of the four lies side by side.
-// ROW_ITEMS groups a lane in flight.  Both directions of 67 million bfloat16 elements in rows of 1000: 91 us (4.5 TB/s; eight lanes
-// of four elements took 109), of 250: 115 us; odd widths move single bytes: 203 us in rows of 251.  Every lane of a warp takes part
+// ROW_ITEMS groups a lane in flight.  Both directions of 67 million bfloat16 elements in rows of 1000: 90 us (4.5 TB/s; eight lanes
+// of four elements took 109), of 250: 113 us; odd widths move single bytes: 201 us in rows of 251.  Every lane of a warp takes part
 // in the shuffles; the ones past the end hold nothing.
 constexpr int ROW_ITEMS = 2, LANE_ELEMS = 8, GROUP_LANES = PACK_GROUP / LANE_ELEMS;
 constexpr int ROW_GROUPS = PACK_THREADS / GROUP_LANES;                 // groups a block and item
 
-// n / d for n < 2^31 without a division: (high word of n m, plus n) >> s
+// n / d for n < 2^31 without a division: (high word of n m, plus n) >> s, with 2^s the power of two at or above d and
+// m = floor(2^32 (2^s - d) / d) + 1 (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994)
 struct FastDiv {
   uint32_t d, m, s;
   explicit FastDiv(uint32_t d_) : d(d_), s(0) {

@@ -160,7 +160,7 @@ class BlockStack(nn.Module):
     def set_checkpoint(self, mode):
         """``"int8"``: a training forward keeps of each block its input alone, in eight bits an element (`pack_activation`), and the
         backward pass runs the block again from it; None: every block keeps what its backward needs.  The gradients are then those of
-        the blocks at the restored inputs (off by at most 1/127 of the largest of each 32 channels).  Blocks run one after another, each
+        the blocks at the restored inputs (off by at most 1/127.5 of the largest of each 32 channels).  Blocks run one after another, each
         taking its norm from the stream as it is stored: outputs are those of the blocks called one by one, bit for bit.  That is also
         what a stack of plain blocks gives without the mode; in a stack of joining blocks the ordinary call forms each norm from the
         stream before its rounding, so that there outputs differ by that rounding (in bfloat16 2^-8 of each element before a norm).
