@@ -4,8 +4,8 @@
 //
 // One CTA owns (batch, head, segment) and walks the chunks of its segment:
 //   S1[t,s] = q'_t . k'_s                      128 x 128 x X   both operands as TMA wrote them
-//   P[t,s]  = S1[t,s] a^{c-s} (s <= t, else 0) -> bfloat16     the only rounding of the part inside the chunk (sequences
-//                                                              of at most 32 tokens: in two parts)
+//   P[t,s]  = S1[t,s] a^{c-s} (s <= t, else 0) -> bfloat16     the only rounding of the part inside the chunk (the rows that
+//                                                              a pass begins with, 32 at least: in two parts)
 //   O[t,e]  = P v' + q' Zb^T                   128 x E x (128 + X)   P read from TMEM; Zb = a^{c+1} s_in / s_out Z rounded to
 //                                                              bfloat16, the only rounding of that part
 //   dZ[e,x] = sum_s (f_s v'_s[e]) k'_s[x]      128 x X x 384   f_s v' in three bfloat16 parts (their sum is it to 2^-25),
@@ -44,6 +44,7 @@ using namespace tc;
 constexpr int LT_T = 128;
 constexpr int LT_W_STATE = 4, LT_W_V = 12, LT_W_OUT = 20, LT_W_LOAD = 24, LT_THREADS = 28 * 32;   // first warps of the roles
 constexpr uint32_t LT_S1 = 0, LT_P = 0, LT_O = 128, LT_DZ = 256, LT_V = 384;   // TMEM columns: 128, 128, 128 and two sets of 3 x 16 (in 512)
+constexpr uint32_t LT_REST = LT_V + 48, LT_REST_STRIDE = 64;   // 16 columns behind either set: the second parts of P
 constexpr int LT_STAGE = 6;                                  // blocks of 16 KB in a stage: q' 2, k' 2, v' 2
 constexpr int LT_SMEM = (2 * LT_STAGE + 2) * (int)BLK + 1024;
 constexpr int LT_FWD_C = 64, LT_REV_C = 63;                  // the token that decays are counted from
@@ -133,9 +134,13 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3;
   const int s0 = seg * p.seg_len, s1 = min(p.L, s0 + p.seg_len), nch = (s1 - s0 + LT_T - 1) / LT_T;
   const int xblocks = X > 64 ? 2 : 1, eblocks = E > 64 ? 2 : 1;   // a narrow head's second blocks are never loaded nor read
-  // A sequence of one slab of 32 tokens: P's sums have too few terms for its roundings to average out, so it keeps the rest of the
-  // rounding as well, in the place of the next slab, which is empty (k-steps 2 and 3, over the same tokens).
-  const bool brief = !local && p.L <= 32;
+  // Where the pass over the sequence begins, P keeps the rest of its rounding as a second part: the scores among the first 32 tokens
+  // (backwards in time: among the last two slabs, which hold the last 32 tokens of a ragged chunk).  Without a state these rows are
+  // then rounded once, as the step's are, however many tokens follow.  It is two to four MMAs a sequence; of the whole of P it would
+  // be 8 in every chunk: [8, 4096, 16, 128, 128] 138 us instead of 117 and backward 388 instead of 336, for an error of 1.33 times
+  // the output rounding's own instead of 1.41 (Zb's rounding remains).
+  const bool opens = !local && seg == (rev ? p.nseg - 1 : 0);
+  const int rest_to = rev ? (min(LT_T, s1 - s0 - (nch - 1) * LT_T) - 1) >> 5 : 0, rest_from = rev ? max(rest_to - 1, 0) : 0;   // slabs
   // The state-only launch has room for two accumulators of dZ in the places of S1 and O: the next product need not wait for the state.
   constexpr int SETS = local ? 2 : 1;
   auto dz_column = [](int c) { return local ? (uint32_t)(c & 1) * 128u : LT_DZ; };
@@ -251,7 +256,13 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
           if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
-              if (!brief || ks < 4) umma_bf16_ta_h(tbase + LT_O, tbase + LT_P + ks * 8, bv + (brief ? inc_mn(ks & 1) : inc_mn(ks)), id_o, 1u);
+              umma_bf16_ta_h(tbase + LT_O, tbase + LT_P + ks * 8, bv + inc_mn(ks), id_o, 1u);
+            if (c == 0 && opens) {
+              for (int j = rest_from; j <= rest_to; ++j)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+                  umma_bf16_ta_h(tbase + LT_O, tbase + LT_REST + (j - rest_from) * LT_REST_STRIDE + ks * 8, bv + inc_mn(2 * j + ks), id_o, 1u);
+            }
             umma_commit(&bars.p_empty);
             umma_commit(&bars.acc_full);
           }
@@ -314,7 +325,7 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
             if (rev ? j < q : j > q) {                       // wholly beyond the diagonal
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = 0u;
-              if (brief) tmem_st16(tmem_addr(tbase, q * 32, LT_P + 16), o);
+              if (c == 0 && opens && j >= rest_from && j <= rest_to) tmem_st16(tmem_addr(tbase, q * 32, LT_REST + (j - rest_from) * LT_REST_STRIDE), o);
             } else {
               uint32_t r[32];
               tmem_ld32(tmem_addr(tbase, q * 32, LT_S1 + j * 32), r);
@@ -344,19 +355,19 @@ __device__ __forceinline__ void la_tc_walk(const LaTcArgs& a, LtShared& sh, uint
               }
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = pack_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-              if (brief) {
+              if (c == 0 && opens && j >= rest_from && j <= rest_to) {
+                const bool keeps = q >= rest_from && q <= rest_to;   // the other rows' scores with these tokens stay as they are
                 uint32_t rest[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                   float lo, hi;
                   unpack_bf16(o[i], lo, hi);
-                  rest[i] = pack_bf16(__uint_as_float(r[2 * i]) - lo, __uint_as_float(r[2 * i + 1]) - hi);
+                  rest[i] = keeps ? pack_bf16(__uint_as_float(r[2 * i]) - lo, __uint_as_float(r[2 * i + 1]) - hi) : 0u;
                 }
-                tmem_st16(tmem_addr(tbase, q * 32, LT_P + 16), rest);
+                tmem_st16(tmem_addr(tbase, q * 32, LT_REST + (j - rest_from) * LT_REST_STRIDE), rest);
               }
             }
             tmem_st16(tmem_addr(tbase, q * 32, LT_P + j * 16), o);
-            if (brief) break;
           }
           tmem_st_wait();
         }
