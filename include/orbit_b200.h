@@ -409,8 +409,8 @@ int orbit_block_norm_bwd(const void* x, int64_t x_row_stride, const void* h, int
 /* ---- activations in eight bits ------------------------------------------------------------------------------------------
  * x [M, D] (row stride in elements) -> q [M, D] signed bytes, exponent [M, ceil(D / 32)] bytes (e + 127 for each 32
  * consecutive elements of a row): x ~ q 2^e with the least e >= -126 for which the group's largest |x| rounds to at most 127.
- * Codes of the largest step 2^122 end at +-63 (the restored value stays finite).  The code -128 marks a non-finite element and is restored as NaN.  Restoring is exact in either dtype.  No counterpart in the
- * reference. */
+ * Codes of the largest step 2^122 end at +-63 (the restored value stays finite).  The code -128 marks a non-finite element and
+ * is restored as NaN.  Restoring is exact in either dtype.  No counterpart in the reference. */
 int orbit_act_pack(const void* x, int64_t x_row_stride, void* q, void* exponent, int64_t M, int D, int dtype, void* stream);
 int orbit_act_unpack(const void* q, const void* exponent, void* x, int64_t M, int D, int dtype, void* stream);
 

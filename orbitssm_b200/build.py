@@ -71,9 +71,9 @@ def build_host(force: bool = False) -> str:
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(shutil.which(nvcc) or "/usr/local/cuda/bin/nvcc")))
     inc = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            os.path.join(cuda, "include")]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f'-DORBIT_HOST_TAG="{host_tag()}"', *["-I" + i for i in inc], HOST_SRC, "-o", HOST_OUT, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch",
-           "-lc10", "-lc10_cuda"]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DORBIT_HOST_TAG="{host_tag()}"', *["-I" + i for i in inc],
+           HOST_SRC, "-o", HOST_OUT, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("g++ failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
@@ -86,7 +86,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
     try:
         build_host(force)
     except (RuntimeError, OSError, ImportError) as e:
-        warnings.warn(f"the native host calls were not built, the Python host side of the operators serves every call: {e}", RuntimeWarning, stacklevel=2)
+        warnings.warn(f"the native host calls were not built, the Python host side of the operators serves every call: {e}", RuntimeWarning,
+                      stacklevel=2)
     return OUT
 
 

@@ -3,9 +3,9 @@
 // A call of these operators on small inputs (one token, one decode batch) costs the host several times what it costs the GPU;
 // checks and ctypes in Python are most of it (measured on the B200 host, us a call: step 16 -> 8, block norm 17 -> 8, an activation
 // to eight bits and back 21 -> 11; a block norm with its backward pass 200 -> 170, the rest of it autograd's own).
-// Each function here serves the ordinary call and returns None for every other one (a CPU tensor, mixed dtypes, a gradient to
-// record, operands that would have to be copied, ...); the Python operator then takes its own way, which serves the call or refuses
-// it by name.  The kernels and the C-ABI entry points are the same on both ways; this file holds no arithmetic.
+// Each function here serves a call on dense operands and returns None for every other one (a CPU tensor, mixed dtypes, a gradient to
+// record, operands that would have to be copied, and views: the LinearAttention layer's column ranges of one projection among them);
+// the Python operator then takes its own way, which serves the call or refuses it by name.  The kernels and the C-ABI entry points are the same on both ways; this file holds no arithmetic.
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
@@ -359,10 +359,18 @@ PyObject* bind_status(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD("bind", bind),     METHOD("la_step", la_step), METHOD("la_fwd", la_fwd), METHOD("block_norm", block_norm),
-                         METHOD("pack", pack),     METHOD("unpack", unpack),
-                         METHOD("bind_status", bind_status), METHOD("la_bwd", la_bwd), METHOD("block_norm_bwd", block_norm_bwd), {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_orbit_host", "Native host calls of the block operators. " ORBIT_HOST_TAG, -1, methods, nullptr, nullptr, nullptr, nullptr};
+PyMethodDef methods[] = {METHOD("bind", bind),
+                         METHOD("bind_status", bind_status),
+                         METHOD("la_step", la_step),
+                         METHOD("la_fwd", la_fwd),
+                         METHOD("la_bwd", la_bwd),
+                         METHOD("block_norm", block_norm),
+                         METHOD("block_norm_bwd", block_norm_bwd),
+                         METHOD("pack", pack),
+                         METHOD("unpack", unpack),
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_orbit_host", "Native host calls of the block operators. " ORBIT_HOST_TAG,
+                      -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

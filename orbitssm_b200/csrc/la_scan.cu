@@ -359,7 +359,9 @@ int la_plan(const LaArgs& a, bool bwd, int nseg, int seg_len, bool local, LaPlan
 
 // The split that takes the fewest chunk steps on 148 SMs: rounds of CTAs times the chunks of a segment and `setup` steps' worth of
 // prologue and state; for more than one segment also the first launch, which reads half of the operands and costs about half a step
-// for each, and `join` steps for the launch between the two.  At most 32 segments: more would only fill rounds that are full.
+// for each, and `join` steps for the launch between the two.  At most 32 segments: `join` is a constant, and the joining launch walks a
+// head's segments one after another.  A call of few heads then leaves SMs idle ([1, 65536, H, 128, 128] bfloat16: H = 1 104 us on 32
+// CTAs, H = 2 113, H = 4 125, H = 16 340).
 // (Tensor-core tiles, 16 heads of 128 x 128, one segment against the split taken: 2048 tokens 51 us and 47, 8192 tokens 167 and 76,
 // 65536 tokens 1233 and 341.  Float32, [2, 777, 8, 64, 64]: 156 and 53.)
 int la_segments(int64_t units, int L, int chunk, double setup, double join, int* seg_len, double* cost_out) {

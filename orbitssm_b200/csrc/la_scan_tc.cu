@@ -17,13 +17,17 @@
 // accumulator and no operand is rounded twice.  That needs a^{-64} to stay far from overflow: heads with a < 1/2 (`steep`) keep
 // a^{t-s} on the scores, where it is at most 1, and their carried part is scaled row by row in TMEM before P v' joins it.
 //
-// What bounds it is the rate of the MMAs (48 of 128 x 128 x 16 a chunk: 107 cycles each with both operands in shared memory, 74 with
-// one in TMEM; 4100 of the 5600 cycles that a chunk takes) and the power limit, so operands are kept in TMEM where it can hold them: per chunk and head of 128 x 128 the tiles move 96 KB in, 288 KB to the MMAs and 160 KB for the element
-// passes.  (With the parts of f v' in shared memory and 64 channels a CTA it was 800 KB, and 158 us where it now takes 119.)
-// Measured: forward [8, 4096, 16, 128, 128] 114 to 119 us (4.5 to 4.7 TB/s of operands and output), backward 360 us; prompt
-// [1, 65536, 16, 128, 128] 341 us.  Random operands draw 1000 W and the SM clock falls to 1.4 to 1.6 GHz; zeros run 20% faster.
+// What bounds it is no one unit: the chain of hand-overs between the roles within a chunk, and the power limit.  Counted over a
+// forward launch at [8, 2048, 16, 128, 128] (of the cycles that an SM is active): tensor pipe 46 %, shared memory 54 % (30 for
+// the operands of MMAs, 24 for ordinary accesses), issue 48 %.  Operands are kept in TMEM where it can hold them: per chunk and
+// head of 128 x 128 the tiles move 96 KB in, 288 KB to the MMAs and 160 KB for the element passes.  (With the parts of f v' in shared
+// memory and 64 channels a CTA it was 800 KB, and 158 us where it now takes 117.)  72 registers a thread at launch leave the six walks of
+// this kernel 1396 bytes of spill stores and 2732 of loads: a walk compiled alone has 76 / 76, of steep heads 640 / 644, state-only
+// none.
+// Measured: forward [8, 4096, 16, 128, 128] 117 us (4.6 TB/s of operands and output), backward 340 us; prompt
+// [1, 65536, 16, 128, 128] 340 us.  Random operands draw 1000 W and the SM clock falls to 1.4 to 1.6 GHz; zeros run 20% faster.
 // bfloat16 calls that these tiles do not serve take the float32 kernels, which need 80 us for [1, 131, 16, 128, 128] where these
-// need 17, and 3827 us for [8, 4096, 16, 128, 128].
+// need 18, and 3827 us for [8, 4096, 16, 128, 128].
 //
 // Warp-specialised, 28 warps that meet only through mbarriers (every wait bounded):
 //   warps 0..3   decay mask: S1 -> P, in the place of S1 (thread = row t)

@@ -221,8 +221,8 @@ def linear_attention(q, k, v, log_decay, state=None, *, scale=None, return_state
     scores or the state rounded once to bfloat16, float32 sums.  That makes the error of y and of the gradients of q, k and v about 1.4
     times that of their own rounding, at every length; scores are kept in two parts where a pass begins (for y and the gradient of q the
     first 32 tokens, for those of k and v the last 32 as far as they share the last chunk of 128), so that without a state these rows are
-    rounded once.  The state itself is float32 throughout.  Other calls run on float32 kernels.  Values are expected to be finite: a NaN or infinity may reach every
-    output of its head and sequence."""
+    rounded once.  The state itself is float32 throughout.  Other calls run on float32 kernels.  Values are expected to be finite: a NaN
+    or infinity may reach every output of its head and sequence."""
     if differentiated(log_decay):
         _checked(q, k, v, log_decay, state, scale)               # refuses a gradient of it
     if wants_node(q, k, v, state):

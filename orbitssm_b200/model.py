@@ -32,7 +32,8 @@ class RMSNorm(nn.Module):
 
 def _listened(m):
     """Does somebody listen to calls of the module (its hooks, or hooks of every module)?"""
-    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks) or nn.modules.module._has_any_global_hook()
+    own = m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+    return bool(own) or nn.modules.module._has_any_global_hook()
 
 
 def _plain(m, cls):
