@@ -356,7 +356,8 @@ int orbit_cp_state_combine(const float* records, int64_t stride, int world, int 
  *   S_t = a S_{t-1} + v_t k_t^T,   y_t = scale S_t q_t,   a = exp(log_decay[h]),   S [B, H, Dv, Dk] fp32 (NULL state0 = zeros)
  * q, k [B, L, H, Dk], v, y [B, L, H, Dv] in the IO dtype with element strides (batch, token, head; the last axis is dense);
  * log_decay [H] fp32, at most 0, a constant (no gradient).  Head widths 1..256; bfloat16 with widths that are multiples of 8 up
- * to 128, 16-byte aligned pointers and strides that are multiples of 8 runs on tcgen05 tiles, everything else on fp32 kernels.
+ * to 128, 16-byte aligned pointers, strides that are multiples of 8 and |scale| within 2^-40 to 2^40 runs on tcgen05 tiles, everything
+ * else on fp32 kernels.
  * Backward reads q, k, v, dy, state0 and dstate1 (gradient of the state after the sequence, NULL = zeros), writes dq, dk, dv
  * and dstate0 (NULL = not wanted).  `status` (device int or NULL) is set if a bounded device wait gave up.  L = 0 passes the
  * state through.  Outputs must not overlap inputs.  No counterpart in the reference, whose scans share their maps over heads

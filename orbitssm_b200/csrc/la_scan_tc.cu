@@ -663,8 +663,11 @@ static bool tc_operand(const void* ptr, int64_t bs, int64_t ls, int64_t hs) {
          hs < (1LL << 38);
 }
 
+// Row factors and the kept state hold scale (or its reciprocal) times a^64 and more, 2^-65 at the least: a scale beyond 2^+-40 could leave
+// the range of float32 with them, and goes to the float32 kernels, whose factors are at most 1.
 bool la_tc_serves(const LaArgs& a, bool bwd, int dtype) {
   if (dtype != BF16 || a.Dk % 8 || a.Dv % 8 || a.Dk > 128 || a.Dv > 128) return false;
+  if (!(fabsf(a.scale) >= 0x1p-40f && fabsf(a.scale) <= 0x1p40f)) return false;
   bool ok = tc_operand(a.q, a.q_bs, a.q_ls, a.q_hs) && tc_operand(a.k, a.k_bs, a.k_ls, a.k_hs) && tc_operand(a.v, a.v_bs, a.v_ls, a.v_hs);
   if (!bwd) return ok && tc_operand(a.y, a.y_bs, a.y_ls, a.y_hs);
   return ok && tc_operand(a.dy, a.dy_bs, a.dy_ls, a.dy_hs) && tc_operand(a.dq, a.dq_bs, a.dq_ls, a.dq_hs) &&

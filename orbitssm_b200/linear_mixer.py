@@ -217,7 +217,7 @@ def linear_attention(q, k, v, log_decay, state=None, *, scale=None, return_state
     scale: default Dk^-0.5.  Returns y [B, L, H, Dv] in the dtype of q, or (y, state after the sequence) with
     `return_state`.  L may be 0.  First-order differentiable in q, k, v and state, through y and the returned state.
 
-    bfloat16 heads whose widths are multiples of 8 up to 128 run on tensor-core tiles: products of the unrounded inputs with the
+    bfloat16 heads whose widths are multiples of 8 up to 128 run on tensor-core tiles (scales within 2^-40 to 2^40): products of the unrounded inputs with the
     scores or the state rounded once to bfloat16, float32 sums.  That makes the error of y and of the gradients of q, k and v about 1.4
     times that of their own rounding, at every length; scores are kept in two parts where a pass begins (for y and the gradient of q the
     first 32 tokens, for those of k and v the last 32 as far as they share the last chunk of 128), so that without a state these rows are

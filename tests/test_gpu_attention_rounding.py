@@ -37,3 +37,21 @@ def test_tokens_after_a_row_do_not_change_it():
     whole = ob.linear_attention(q, k, v, ld)
     for n in (1, 2, 31, 32, 33):
         assert torch.equal(ob.linear_attention(q[:, :n], k[:, :n], v[:, :n], ld)[:, :32], whole[:, :min(n, 32)])
+
+
+@pytest.mark.parametrize("scale", [1e-30, 2.0 ** -41, 2.0 ** -40, -2.0 ** -39, 2.0 ** 40, -2.0 ** 41, 1e20, 1e30])
+@pytest.mark.parametrize("L", [20, 200])
+def test_any_scale_that_float32_holds(L, scale):
+    q, k, v, _, s0, dy, ds1 = _inputs(1, L, 3, 64, 72, BF, 57)
+    ld = torch.tensor([-0.69, -0.8, -0.01], device=DEV)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v, s0)]
+    y, s1 = ob.linear_attention(*leaves[:3], ld, leaves[3], scale=scale, return_state=True)
+    got = [y, s1, *torch.autograd.grad((y, s1), leaves, (dy, ds1))]
+    want, big = ref_attention(q, k, v, ld, s0, scale, dy, ds1), majorant(q, k, v, ld, s0, scale, dy, ds1)
+    for i, (a, b, m) in enumerate(zip(got, want, big, strict=True)):
+        u, op = (2.0 ** -24, 0.0) if i in (1, 5) else (2.0 ** -8, 2.0 ** -8)
+        # the bound of the other tests, in the units of the largest sum: at 1e-30 their absolute slack would hide a result of zeros
+        unit = float(m.max())
+        err = (a.double() - b).abs() / unit
+        assert bool((err <= (u * b.abs() + (op + 600 * 2.0 ** -24) * m) / unit).all()), i
+    ops.check_device_status()
