@@ -14,8 +14,10 @@
 //   out = s_out a^{t-c} O;   Z = a^T Z + dZ                    Z [e, x] in registers, float32
 // The decay a^{t-s} is split into a column factor on the scores and a row factor on the float32 accumulator, counted from the
 // middle of the chunk (c = 64; backwards in time a^{s-c} and a^{c-t}, c = 63), so that both parts of the output meet in one
-// accumulator and no operand is rounded twice.  That needs a^{-64} to stay far from overflow: heads with a < 1/2 (`steep`) keep
-// a^{t-s} on the scores, where it is at most 1, and their carried part is scaled row by row in TMEM before P v' joins it.
+// accumulator and no operand is rounded twice.  It also takes a^{64} of the range of float32 at either end, so heads with
+// a < 2^{-1/2} (`steep`) keep a^{t-s} on the scores, where it is at most 1, and their carried part is scaled row by row in TMEM before
+// P v' joins it ([8, 4096, 16, 128, 128] forward 164 us instead of 118, backward 499 instead of 340; with the limit at 1/2 values of
+// 2^80 gave NaN there, and gradients of 2^-60 lost the state's).
 //
 // What bounds it is no one unit: the chain of hand-overs between the roles within a chunk, and the power limit.  Counted over a
 // forward launch at [8, 2048, 16, 128, 128] (of the cycles that an SM is active): tensor pipe 46 %, shared memory 54 % (30 for
@@ -100,7 +102,7 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, const void* s
                "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
-// a^n for |n| <= 128 from the table of a^0 .. a^128 (n < 0 only where a is at least 1/2)
+// a^n for |n| <= 128 from the table of a^0 .. a^128 (n < 0 only where a is at least 2^{-1/2})
 __device__ __forceinline__ float power(const float* pw, int n) { return n >= 0 ? pw[n] : __fdividef(1.f, pw[-n]); }
 
 // One lane of a converged warp, the same one every time.  Issued under a plain `lane == 0` test the compiler takes the MMA's
@@ -644,7 +646,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   if (local && seg == (rev ? 0 : p.nseg - 1)) return;        // nobody reads the last segment's share
   uint8_t* sm = align1024(smem_raw);
   const double ld = (double)p.log_decay[h];
-  const bool steep = !(fabs(ld) <= 0.693147);
+  const bool steep = !(fabs(ld) <= 0.346573);                // a at least 2^{-1/2}
   if (local) {
     if (rev) la_tc_walk<true, false, true>(a, sh, sm, jb, b, h, seg, et, ld);
     else la_tc_walk<false, false, true>(a, sh, sm, jb, b, h, seg, et, ld);
@@ -663,7 +665,7 @@ static bool tc_operand(const void* ptr, int64_t bs, int64_t ls, int64_t hs) {
          hs < (1LL << 38);
 }
 
-// Row factors and the kept state hold scale (or its reciprocal) times a^64 and more, 2^-65 at the least: a scale beyond 2^+-40 could leave
+// Row factors and the kept state hold scale (or its reciprocal) times a^64 and more, 2^-33 at the least: a scale beyond 2^+-40 could leave
 // the range of float32 with them, and goes to the float32 kernels, whose factors are at most 1.
 bool la_tc_serves(const LaArgs& a, bool bwd, int dtype) {
   if (dtype != BF16 || a.Dk % 8 || a.Dv % 8 || a.Dk > 128 || a.Dv > 128) return false;

@@ -55,3 +55,22 @@ def test_any_scale_that_float32_holds(L, scale):
         err = (a.double() - b).abs() / unit
         assert bool((err <= (u * b.abs() + (op + 600 * 2.0 ** -24) * m) / unit).all()), i
     ops.check_device_status()
+
+
+@pytest.mark.parametrize("powers", [(0, 0, -60, 0), (0, 0, 0, -60), (0, 0, 80, 0), (0, 0, 0, 80), (20, 20, 20, 20), (-20, -20, -20, -20)])
+def test_values_far_from_one(powers):
+    """Every head takes its decays without leaving the range of float32 where the operator's own terms are in it."""
+    L, H, D = 200, 6, 64
+    q, k, v, _, s0, dy, ds1 = _inputs(1, L, H, D, D, BF, 58)
+    ld = torch.tensor([-0.01, -0.2, -0.3465, -0.3467, -0.5, -0.69], device=DEV)
+    q, k, v, dy = (t * 2.0 ** e for t, e in zip((q, k, v, dy), powers))
+    s0, ds1 = s0 * 2.0 ** (powers[1] + powers[2]), ds1 * 2.0 ** (powers[0] + powers[3])
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v, s0)]
+    y, s1 = ob.linear_attention(*leaves[:3], ld, leaves[3], return_state=True)
+    got = [y, s1, *torch.autograd.grad((y, s1), leaves, (dy, ds1))]
+    want, big = ref_attention(q, k, v, ld, s0, D ** -0.5, dy, ds1), majorant(q, k, v, ld, s0, D ** -0.5, dy, ds1)
+    for i, (a, b, m) in enumerate(zip(got, want, big, strict=True)):
+        u, op = (2.0 ** -24, 0.0) if i in (1, 5) else (2.0 ** -8, 2.0 ** -8)
+        unit = float(m.max())
+        assert bool(((a.detach().double() - b).abs() / unit <= (u * b.abs() + (op + 600 * 2.0 ** -24) * m) / unit).all()), i
+    ops.check_device_status()
