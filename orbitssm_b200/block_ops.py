@@ -192,6 +192,8 @@ def _block_norm(x, h, gate, scale, w_post, w_pre, eps, keep):
     r, n, rh, rr = block_norm_fwd(x2, h2, g2, s32, wo, wi, eps, keep)
     if x.dim() != 2:
         r, n = r.view(x.shape), None if n is None else n.view(x.shape)
+        # kept in the shape that the native call keeps: a run again on the other host way saves the like
+        x2, h2, g2 = (None if t is None else t.view(x.shape) for t in (x2, h2, g2))
     return r, n, (x2, h2, g2, s32, wo, wi, rh, rr)
 
 

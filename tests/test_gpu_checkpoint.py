@@ -94,3 +94,23 @@ def test_outputs_with_and_without_the_checkpoint(dtype):
     u = torch.finfo(dtype).eps / 2
     # (float32: the sum of the 64 squares and the product with the weight add their own roundings, fewer than 64)
     assert bool(((got - want).abs() <= (4.1 * u + 64 * 2.0 ** -24) * want.abs()).all())
+
+
+def test_the_two_runs_of_a_block_may_take_either_host_way():
+    stack = stack_of(post_norm=True, gate=True, residual_scale=0.5)
+    x = torch.randn(2, 40, 64, device=DEV)
+
+    def grads(timed_first, timed_second):
+        stack.zero_grad(set_to_none=True)
+        try:
+            ops.set_timing([] if timed_first else None)                  # a timed region takes the Python way
+            y = stack(x)
+            ops.set_timing([] if timed_second else None)
+            y.square().sum().backward()
+        finally:
+            ops.set_timing(None)
+        return [p.grad.clone() for p in stack.parameters()]
+
+    want = grads(False, False)
+    for a, b in ((True, False), (False, True), (True, True)):
+        assert all(torch.equal(g, w) for g, w in zip(grads(a, b), want))
