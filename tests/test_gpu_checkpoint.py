@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import orbitssm_b200 as ob
+from conftest import load_golden
 from orbitssm_b200 import ops
 from orbitssm_b200.block_ops import checkpoint_block
 
@@ -114,3 +115,36 @@ def test_the_two_runs_of_a_block_may_take_either_host_way():
     want = grads(False, False)
     for a, b in ((True, False), (False, True), (True, True)):
         assert all(torch.equal(g, w) for g, w in zip(grads(a, b), want))
+
+
+def _other_mixer(name):
+    if name == "hybrid":
+        return ob.HybridMambaSSM(ob.HybridMambaConfig(**load_golden("hm_small")["config"]))
+    if name == "ssd":
+        return ob.SSDMimoSSM(ob.mamba2_config(64, d_state=16, d_head=16))
+    if name == "ssd tiles":
+        return ob.SSDMimoSSM(ob.mamba2_config(128, d_state=128, d_head=64))
+    return mixer(128)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kw", [dict(), dict(post_norm=True, residual_scale=0.5)])
+@pytest.mark.parametrize("name", ["ssd", "ssd tiles", "hybrid", "linear"])
+def test_gradients_at_inputs_that_eight_bits_hold_are_the_blocks_own(name, kw, dtype):
+    """Whole numbers up to 127 are restored as they were: gradients, hooks or not, have to be those of the block without a checkpoint."""
+    torch.manual_seed(7)
+    m = _other_mixer(name)
+    stack = ob.BlockStack.from_mixers([m], m.d_model, **kw).to(DEV).to(dtype)
+    x = torch.randint(-127, 128, (2, 150, m.d_model), device=DEV).to(dtype)
+    dy = torch.randn(x.shape, device=DEV).to(dtype)
+
+    def run(block):
+        for p in stack.parameters():
+            p.grad = None
+        xx = x.clone().requires_grad_(True)
+        block(xx).backward(dy)
+        return [xx.grad, *[p.grad for p in stack.layers[0].parameters()]]
+
+    got, want = run(lambda t: checkpoint_block(stack.layers[0], t)), run(stack.layers[0])
+    assert all((a is None) == (b is None) and (a is None or torch.equal(a, b)) for a, b in zip(got, want, strict=True))
+    ops.check_device_status()
