@@ -262,6 +262,8 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out_state=No
         state = state.contiguous()
     if out_state is not None and out_state.data_ptr() != state.data_ptr() and _overlap(out_state, state):
         raise ValueError(f"{who}: out_state overlaps state without being it")
+    if out_state is not None and any(_overlap(out_state, t) for t in (q, k, v, log_decay)):
+        raise ValueError(f"{who}: out_state overlaps q, k, v or log_decay")
     new = torch.empty_like(state) if out_state is None else out_state
     if out_state is not None and not out_state.is_inference():
         torch.autograd.graph.increment_version(out_state)        # a graph that kept it must not read the new one
@@ -280,9 +282,16 @@ def _dense_rows(t):
     return t if t.shape[2] == 1 or t.stride(2) == 1 else t.contiguous()
 
 
+def _extent(t):
+    """The bytes from a tensor's first element to its last."""
+    if t.numel() == 0:
+        return 0, 0
+    return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
 def _overlap(a, b):
-    n = a.numel() * 4
-    return a.data_ptr() < b.data_ptr() + n and b.data_ptr() < a.data_ptr() + n
+    (a0, a1), (b0, b1) = _extent(a), _extent(b)
+    return a0 < b1 and b0 < a1
 
 
 # ----------------------------------------------------------------------------------------------------

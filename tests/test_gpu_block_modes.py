@@ -84,3 +84,19 @@ def test_without_the_host_call_module_the_results_are_the_same_bits(monkeypatch)
     want = run()
     monkeypatch.setattr(_lib, "_host", _lib._PythonSide())
     assert all(torch.equal(a, b) for a, b in zip(run(), want, strict=True))
+
+
+def test_a_new_state_written_over_an_operand_is_refused():
+    q, k, v, ld, s, _, _ = _args(1)
+    arena = torch.zeros(4096, device=DEV)
+    state = arena[:s.numel()].view(s.shape)
+    for i, (name, t) in enumerate((("q", q), ("k", k), ("v", v))):
+        ops = [q[:, 0], k[:, 0], v[:, 0]]
+        ops[i] = arena[s.numel() - 4:][:t.numel()].view(t[:, 0].shape)
+        with pytest.raises(ValueError, match="out_state overlaps q, k, v or log_decay"):
+            ob.linear_attention_step(*ops, ld, s, out_state=state)
+        ops[i] = arena[s.numel():][:t.numel()].view(t[:, 0].shape)        # beside it: served
+        _, new = ob.linear_attention_step(*ops, ld, s, out_state=state)
+        assert new is state and bool(torch.isfinite(new).all())
+    with pytest.raises(ValueError, match="out_state overlaps q, k, v or log_decay"):
+        ob.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], arena[5:7], s, out_state=state)
