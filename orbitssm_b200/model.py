@@ -66,6 +66,7 @@ class ResidualBlock(nn.Module):
         self.scale = None if residual_scale is None else nn.Parameter(torch.full((d_model,), float(residual_scale)))
 
     n_residuals = 1
+    joins = False                        # (a block that was pickled before there were any has no such entry)
 
     def join(self, x, n, h, next_norm=None):
         """(x + scale * post_norm(h) * sigmoid(gate_proj(n)), next_norm of it | None) in one kernel."""
@@ -139,6 +140,8 @@ def _joins(block):
 
 
 class BlockStack(nn.Module):
+    checkpoint = None
+
     def __init__(self, blocks, d_model, *, residual_rescale=True):
         super().__init__()
         self.layers = nn.ModuleList(blocks)

@@ -167,3 +167,19 @@ def test_a_block_of_its_own_forward_is_called():
     stack = make()
     stack.layers[1] = Doubled(Mix(), D, post_norm=True).double()
     check(stack)
+
+
+def test_a_stack_pickled_before_blocks_could_join_still_runs():
+    stack = make(post_norm=False, gate=False, residual_scale=None)
+    for b in stack.layers:
+        del b.__dict__["joins"]
+        for name in ("post_norm", "gate_proj", "scale"):                  # attributes that such a block does not have
+            b.__dict__.pop(name, None), b._modules.pop(name, None), b._parameters.pop(name, None)
+    del stack.__dict__["checkpoint"]
+    x = torch.randn(2, 5, D, dtype=torch.float64)
+    want = x
+    for b in stack.layers:
+        want = want + b.mixer(b.norm(want))
+    want = stack.norm_f(want)
+    assert torch.equal(stack(x), want) and torch.equal(stack(x, return_state=True)[0], want)
+    assert torch.allclose(stack.step(x[:, 0], [None] * 3)[0], want[:, 0], rtol=1e-12, atol=1e-12)
