@@ -54,8 +54,8 @@ def launch(name, launches, device, fn, *args):
 
 def native(name, *args):
     """The outputs of host call `name` (`_lib.host`), or None where it leaves the call to the Python way."""
-    if ops._TIMING is not None or forward_ad._current_level >= 0 or tracing():
-        return None                    # a timed region needs the events around the launch, the others the checks of the Python way
+    if ops._TIMING is not None:
+        return None                    # a timed region needs the events around the launch
     got = getattr(_lib._host or _lib.host(), name)(*args)
     if got is None:
         return None

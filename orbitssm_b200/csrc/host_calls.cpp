@@ -8,6 +8,7 @@
 // the Python operator then takes its own way, which serves the call or refuses it by name.  The kernels and the C-ABI entry points are the same on both ways; this file holds no arithmetic.
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -36,20 +37,23 @@ struct Entry {
   decltype(&orbit_act_unpack) unpack;
 } entry = {};
 
-// a plain torch.Tensor (no subclass) on the current CUDA device for which no gradient is to be recorded
+// a plain torch.Tensor (no subclass) on the current CUDA device for which no gradient is to be recorded and that carries no
+// forward-mode tangent
 bool plain(PyObject* o, at::Tensor& t, int device) {
   if (!THPVariable_CheckExact(o)) return false;
   t = THPVariable_Unpack(o);
-  return t.is_cuda() && t.get_device() == device && !(t.requires_grad() && c10::GradMode::is_enabled()) && t.layout() == at::kStrided;
+  return t.is_cuda() && t.get_device() == device && !(t.requires_grad() && c10::GradMode::is_enabled()) && t.layout() == at::kStrided &&
+         !t._fw_grad(0).defined();
 }
 bool plain_or_none(PyObject* o, at::Tensor& t, int device) { return o == Py_None || plain(o, t, device); }
 
 int io_code(const at::Tensor& t) {
   return t.scalar_type() == at::kBFloat16 ? ORBIT_BF16 : t.scalar_type() == at::kFloat ? ORBIT_F32 : -1;
 }
-// the current device, or -1 for a call whose first operand does not live on a CUDA device (there may be none at all)
+// the current device, or -1 for a call whose first operand does not live on a CUDA device (there may be none at all) and for one that
+// torch.jit.trace records
 int device_for(PyObject* first) {
-  if (c10::impl::dispatch_mode_enabled() || !THPVariable_CheckExact(first) || !THPVariable_Unpack(first).is_cuda()) return -1;
+  if (c10::impl::dispatch_mode_enabled() || at::tracer::impl::is_dispatch_enabled() || !THPVariable_CheckExact(first) || !THPVariable_Unpack(first).is_cuda()) return -1;
   return c10::cuda::current_device();
 }
 void* stream(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
