@@ -180,7 +180,7 @@ class SplitColumnsFn(torch.autograd.Function):
         ref = next(g for g in grads if g is not None)
         arena = ctx.arena
         if arena is not None and arena.buf is not None and arena.buf.dtype == ref.dtype:
-            out = arena.buf
+            out, arena.buf = arena.buf, None       # the gradient's alone from here on: a graph that is kept holds no buffer
         else:
             out = torch.empty(ctx.shape, device=ref.device, dtype=ref.dtype)
         o = 0
