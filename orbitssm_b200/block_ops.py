@@ -9,7 +9,6 @@ import weakref
 from typing import NamedTuple
 
 import torch
-import torch.utils.checkpoint
 from torch.autograd import forward_ad
 
 from . import _lib, ops
@@ -362,8 +361,10 @@ class _Drawn:
         self.states = [g.get_state() for g in self.generators]
 
     def note(self, block):
-        if len(self.generators) == 2:
-            _DRAWS.setdefault(block, {})[_flags(block)] = not torch.equal(self.generators[1].get_state(), self.states[1])
+        drew = [not torch.equal(g.get_state(), s) for g, s in zip(self.generators, self.states)]
+        if len(drew) == 2:
+            _DRAWS.setdefault(block, {})[_flags(block)] = drew[1]
+        self.generators, self.states = ([x for x, d in zip(xs, drew) if d] for xs in (self.generators, self.states))
 
     def __enter__(self):
         self.found = [g.get_state() for g in self.generators]
@@ -375,29 +376,58 @@ class _Drawn:
             g.set_state(s)
 
 
+class _Checkpoint:
+    """A block's run whose saved tensors are dropped (`drop` gives autograd a number for each) and formed again by a second run when
+    the backward pass asks for the first of them (`fetch`)."""
+
+    def __init__(self, block, x):
+        params = list(block.parameters())
+        self.block, self.packed, self.wanted = block, pack_activation(x), x.requires_grad
+        self.versions = [(p, p._version) for p in params if not p.is_inference()]
+        self.autocast = dict(dtype=torch.get_autocast_dtype("cuda"), enabled=torch.is_autocast_enabled("cuda"), cache_enabled=False)
+        self.saved = []                  # shape, dtype and device of each
+        self.again = {}                  # number -> tensor of the second run, until it is fetched
+        self.drawn = _Drawn(block, x.device)
+
+    def first(self, x):
+        with torch.autograd.graph.saved_tensors_hooks(self.drop, self.fetch):
+            y = self.block(x)
+        self.drawn.note(self.block)
+        return y
+
+    def drop(self, t):
+        self.saved.append((t.shape, t.dtype, t.device))
+        return len(self.saved) - 1
+
+    def fetch(self, i):
+        if i not in self.again:          # (also where a kept graph is walked once more)
+            self.again = self.second()
+        return self.again.pop(i)
+
+    def second(self):
+        for p, version in self.versions:
+            if p._version != version:
+                raise RuntimeError(f"8-bit activation checkpoint: a parameter {tuple(p.shape)} that the block's backward pass needs was "
+                                   f"modified by an inplace operation (version {p._version}, expected {version})")
+        kept = []
+        keep = torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.detach()), _never)
+        with torch.enable_grad(), torch.autocast("cuda", **self.autocast), self.drawn, keep:
+            self.block(unpack_activation(self.packed).requires_grad_(self.wanted))
+        if [(t.shape, t.dtype, t.device) for t in kept] != self.saved:
+            raise RuntimeError("8-bit activation checkpoint: the block's second run saved other tensors for its backward pass than its first "
+                               f"({len(kept)} and {len(self.saved)} of them): its course has to depend on its input's shape alone")
+        return dict(enumerate(kept))
+
+
+def _never(t):
+    raise RuntimeError("8-bit activation checkpoint: the graph of a block's second run is not differentiated")
+
+
 def checkpoint_block(block, x):
     """``block(x)`` without keeping what the block's backward needs: its input waits in eight bits, and the backward pass restores
     it, runs the block again from it and differentiates the block's own graph with what that run saves (so that hooks of parameters
     and modules see one backward pass).  The second run draws the random numbers of the first.  Refused: a parameter changed in
     place in between, and a block that draws on the GPU inside a graph capture.  An ordinary call where no gradient is wanted."""
-    params = list(block.parameters())
-    if not torch.is_grad_enabled() or not (x.requires_grad or any(p.requires_grad for p in params)):
+    if not torch.is_grad_enabled() or not (x.requires_grad or any(p.requires_grad for p in block.parameters())):
         return block(x)
-    packed = pack_activation(x)
-    dtype, wanted = x.dtype, x.requires_grad
-    versions = [(p, p._version) for p in params if not p.is_inference()]
-    first, drawn = [x], _Drawn(block, x.device)
-
-    def run(q, exponent):
-        if first:
-            y = block(first.pop())
-            drawn.note(block)
-            return y
-        for p, version in versions:
-            if p._version != version:
-                raise RuntimeError(f"8-bit activation checkpoint: a parameter {tuple(p.shape)} that the block's backward pass needs was "
-                                   f"modified by an inplace operation (version {p._version}, expected {version})")
-        with drawn:
-            return block(unpack_activation(PackedActivation(q, exponent, dtype)).requires_grad_(wanted))
-
-    return torch.utils.checkpoint.checkpoint(run, packed.q, packed.exponent, use_reentrant=False, preserve_rng_state=False)
+    return _Checkpoint(block, x).first(x)

@@ -160,3 +160,35 @@ def test_blocks_that_run_context_parallel_are_refused_whenever_they_were_made_so
     with pytest.raises(ValueError, match="context-parallel"):
         stack.set_checkpoint("int8")
     assert stack.set_checkpoint(None).checkpoint is None
+
+
+def test_a_block_whose_second_run_takes_another_course_is_refused():
+    class Fickle(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.lin, self.calls = nn.Linear(8, 8).double(), 0
+
+        def forward(self, x):
+            self.calls += 1
+            return torch.tanh(self.lin(x)) if self.calls == 1 else self.lin(x)
+
+    y = block_ops.checkpoint_block(Fickle(), _x())
+    with pytest.raises(RuntimeError, match="saved other tensors"):
+        y.sum().backward()
+
+
+def test_what_a_checkpointed_run_keeps_goes_with_its_graph():
+    import gc
+    import weakref
+    block, x = _block(), _x()
+    kept = []
+    fetch = block_ops._Checkpoint.fetch
+    gc.disable()                                                         # by reference counts alone
+    try:
+        block_ops._Checkpoint.fetch = lambda self, i: kept.append(weakref.ref(self)) or fetch(self, i)
+        y = block_ops.checkpoint_block(block, x)
+        y.sum().backward()
+        assert kept and all(r() is None for r in kept)                   # (y is still there: its graph has given up what it saved)
+    finally:
+        block_ops._Checkpoint.fetch = fetch
+        gc.enable()
