@@ -9,6 +9,12 @@ pytestmark = pytest.mark.gpu
 DEV, BF = "cuda", torch.bfloat16
 
 
+@pytest.fixture(autouse=True)
+def _leave_no_cache():
+    yield
+    torch.cuda.empty_cache()
+
+
 def _fill(*shape, dtype=BF, seed=0):
     """Random values, a block of 2^24 repeated (quick to make), the last one anew."""
     g = torch.Generator(device=DEV).manual_seed(seed)
