@@ -426,8 +426,8 @@ def _never(t):
 def checkpoint_block(block, x):
     """``block(x)`` without keeping what the block's backward needs: its input waits in eight bits, and the backward pass restores
     it, runs the block again from it and differentiates the block's own graph with what that run saves (so that hooks of parameters
-    and modules see one backward pass).  The second run draws the random numbers of the first.  Refused: a parameter changed in
-    place in between, and a block that draws on the GPU inside a graph capture.  An ordinary call where no gradient is wanted."""
+    and modules see one backward pass).  The second run draws the random numbers of the first (from torch's default generators, the
+    CPU's and the input's device's).  Refused: a block that saves other tensors when it runs again, a parameter changed in place in between, and a block that draws on the GPU inside a graph capture.  An ordinary call where no gradient is wanted."""
     if not torch.is_grad_enabled() or not (x.requires_grad or any(p.requires_grad for p in block.parameters())):
         return block(x)
     return _Checkpoint(block, x).first(x)

@@ -20,8 +20,9 @@
 // (no atomics: reproducible).
 //
 // HBM-bound: forward (2 + gate) reads and 2 writes of es bytes an element, backward (4 + gate) reads and (2 + gate) writes.
-// Measured at [65536, 2048] bfloat16 with every factor: forward 227 us (5.9 TB/s, 90 % of the copy bandwidth), backward 419 us
-// (5.1 TB/s, 78 %: one barrier a row at two CTAs of 256 threads an SM, registers allow no third).
+// Measured at [65536, 2048] with every factor: bfloat16 forward 227 us (5.9 TB/s, 90 % of the copy bandwidth), backward 419 us
+// (5.1 TB/s, 78 %: one barrier a row at two CTAs of 256 threads an SM, registers allow no third); float32 497 us (5.4 TB/s) and 716
+// (6.0 TB/s).
 #include "common.cuh"
 #include "../../include/orbit_b200.h"
 
@@ -300,7 +301,8 @@ __global__ void __launch_bounds__(bn_threads(TPR), NV > 1 || TPR > 256 ? 1 : 2) 
 }
 
 // Rows that 16-byte vectors do not divide, or wider than the registers hold: one CTA a row, element by element, the row read
-// again for each sum.
+// again for each sum.  bfloat16 [65536, 1001] forward 600 us and backward 1353 (rows of 1000: 117 and 249), [16384, 9000] 990 us and
+// 2960; float32 669 and 1502, 1305 and 4119.
 template <typename T>
 __global__ void __launch_bounds__(BN_THREADS) block_norm_fwd_scalar_kernel(const BnArgs a) {
   __shared__ float red[32];
@@ -420,7 +422,7 @@ __global__ void __launch_bounds__(256) block_norm_colsum_kernel(const float* __r
 // 16-byte vectors a row takes -> threads a row and vectors a thread (0: the scalar kernels).  A row keeps to one warp up to 32
 // vectors and spreads over up to 512 threads, one vector of each tensor a thread (72 registers forward, 125 to 128 backward), so that
 // many rows are in flight.  Rows of 513 to 1024 vectors take four a thread: 217 registers forward ([16384, 8192] bfloat16 with every
-// factor: 229 us, 5.9 TB/s), 255 backward with 2312 bytes of spill stores and 1424 of loads, which bound it (1710 us, 1.3 TB/s).
+// factor: 229 us, 5.9 TB/s), 255 backward with 2312 bytes of spill stores and 1424 of loads, which bound it (1710 us, 1.3 TB/s; [16384, 5120] 175 and 1050 us).
 struct BnShape { int tpr, nv; };
 static BnShape bn_shape(int vectors) {
   if (vectors <= 32) return {32, 1};

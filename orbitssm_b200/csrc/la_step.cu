@@ -4,7 +4,8 @@
 // product with q is a shuffle sum.  ROWS rows a group keep that many 16-byte loads a thread in flight.  S' may be S itself:
 // every element is read and written by the same thread, read first.
 // HBM-bound: 8 bytes a state element and token.  2048 states of 128 x 128, bfloat16 operands, from memory: 49 us (5.5 TB/s), 8192 of
-// them 174 us (6.2 TB/s, 94% of the measured copy); 2048 states of 96 x 128: 41 us (5.0 TB/s).
+// them 174 us (6.2 TB/s, 94% of the measured copy); 2048 states of 96 x 128: 41 us (5.0 TB/s).  With clean lines in L2 before the call 42
+// us for the first of these, 45 with float32 operands.
 #include "common.cuh"
 #include "../../include/orbit_b200.h"
 

@@ -300,7 +300,9 @@ def _overlap(a, b):
 @dataclass(frozen=True)
 class LinearAttentionConfig:
     """`LinearAttention` layer.  Heads have keys of `d_key` and values of `d_value` channels (default d_model / n_heads
-    each); head h forgets over a span that runs geometrically from `span_min` to `span_max` tokens: decay 1 - 1 / span."""
+    each); head h forgets over a span that runs geometrically from `span_min` to `span_max` tokens: decay 1 - 1 / span.
+    In bfloat16, widths that are multiples of 8 up to 128 run on tensor cores; others (up to 256) take the float32 kernels, which need
+    about 30 times as long."""
     d_model: int
     n_heads: int
     d_key: int | None = None
