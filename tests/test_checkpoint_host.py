@@ -192,3 +192,36 @@ def test_what_a_checkpointed_run_keeps_goes_with_its_graph():
     finally:
         block_ops._Checkpoint.fetch = fetch
         gc.enable()
+
+
+def test_checkpoints_inside_a_checkpointed_block():
+    from torch.utils.checkpoint import checkpoint
+
+    class Outer(nn.Module):
+        def __init__(self, how):
+            super().__init__()
+            self.a, self.b, self.how = _block(1), _block(2), how
+
+        def forward(self, x):
+            if self.how == "torch":
+                return self.b(checkpoint(self.a, x, use_reentrant=False))
+            return self.b(block_ops.checkpoint_block(self.a, x))
+
+    for how in ("torch", "own"):
+        assert _same(Outer(how), _x())
+
+
+def test_a_step_of_two_blocks_with_a_shared_parameter_and_an_accumulated_gradient():
+    a, x = _block(1), _x()
+    want = None
+    for checkpointed in (False, True):
+        for p in a.parameters():
+            p.grad = None
+        for _ in range(2):                                               # gradients add up over two passes
+            y = x
+            for _ in range(2):                                           # the block twice in a row
+                y = block_ops.checkpoint_block(a, y) if checkpointed else a(y)
+            y.sum().backward()
+        got = [p.grad.clone() for p in a.parameters()]
+        want = got if want is None else want
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
